@@ -27,6 +27,7 @@ from .functional import (  # noqa: E402,F401  the rest of the initialisers (endi
     rand_xavier_normal_like, rand_xavier_uniform, rand_xavier_uniform_, rand_xavier_uniform_like, randn_, randn_like,
     randu_, randu_like, zeros_, zeros_like,
 )
+from .functional import attention, linear_cross_entropy, relative_attention  # noqa: E402,F401  operators of sequence models
 from .autograd.functional import backward, grad, hessian, jacobian, value_and_grad  # noqa: E402,F401
 from . import autograd, fusion, graph, nn, optim, utils  # noqa: E402,F401
 from .fusion import fuse  # noqa: E402,F401

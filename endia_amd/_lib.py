@@ -69,6 +69,13 @@ class SgemmDesc(ctypes.Structure):
                 ("bias", c_void_p)]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, c_int64) for n in ("B", "Q", "K", "H", "Hk", "D")] + [
+        (n, c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides")] + [
+        ("query_offset", c_int64), ("scale", c_float), ("causal", c_int32), ("buckets", c_int32), ("max_distance", c_int32),
+        ("both_sides", c_int32)]
+
+
 class ColSumDesc(ctypes.Structure):
     _fields_ = [("R", c_int64), ("C", c_int64), ("x", c_void_p), ("out", c_void_p), ("scale", c_float)]
 
@@ -129,6 +136,10 @@ SIGNATURES = {
     "endia_hip_col_sum_multi": [c_int32, POINTER(ColSumDesc)],
     "endia_hip_reduce": [c_int32, c_int32, _i64p, c_uint32, _fp, _fp],
     "endia_hip_mse_fwd_bwd": [c_int64, _fp, _fp, _fp, _fp],
+    "endia_hip_linear_cross_entropy_fwd": [c_int64, c_int64, c_int64, _fp, c_int64, c_int32, _fp, c_int64, _fp, _fp, _fp],
+    "endia_hip_linear_cross_entropy_bwd": [c_int64, c_int64, c_int64, _fp, c_int64, c_int32, _fp, c_int64, _fp, _fp, _fp, _fp, _fp],
+    "endia_hip_attention_fwd": [POINTER(AttentionDesc), _fp, _fp, _fp, _fp, _fp, _fp, _fp],
+    "endia_hip_attention_bwd": [POINTER(AttentionDesc), _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp],
     "endia_hip_conv2d_out_shape": [POINTER(Conv2dDesc), _i64p, _i64p],
     "endia_hip_conv2d_fwd": [POINTER(Conv2dDesc), _fp, _fp, _fp, _fp, c_int32],
     "endia_hip_conv2d_bwd_data": [POINTER(Conv2dDesc), _fp, _fp, _fp],
@@ -217,6 +228,7 @@ def _raw_call(name, *args):
 _WRITES_FRESH = frozenset({
     "endia_hip_malloc", "endia_hip_free", "endia_hip_binary", "endia_hip_unary_fwd", "endia_hip_unary_vjp",
     "endia_hip_unary_vjp_from_output", "endia_hip_ew_program", "endia_hip_reduce_add", "endia_hip_reduce",
+    "endia_hip_linear_cross_entropy_fwd", "endia_hip_linear_cross_entropy_bwd", "endia_hip_attention_fwd", "endia_hip_attention_bwd",
     "endia_hip_strided_copy", "endia_hip_mse_fwd_bwd", "endia_hip_complex_pack", "endia_hip_linear_bwd",
     "endia_hip_conv2d_out_shape", "endia_hip_conv3d_out_shape", "endia_hip_pool_out_shape",
 })

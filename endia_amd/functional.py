@@ -1320,6 +1320,129 @@ def mse(pred, target):
 
 
 # --------------------------------------------------------------------------------------------------
+# operators of sequence models: no counterpart in the reference, which would spell them in matmul, exp, sum and div
+# --------------------------------------------------------------------------------------------------
+def _first_order_only(name, grad, out):
+    from .autograd.functional import building_graph
+    if building_graph():
+        raise NotImplementedError("%s has no second-order rule" % name)
+    if grad.ndim() != out.ndim():
+        raise NotImplementedError("%s has no rule for a cotangent with leading Jacobian axes (non-scalar output)" % name)
+
+
+def _real_operands(name, *arrays):
+    for a in arrays:
+        if a is not None and a.is_complex_:
+            raise ValueError("%s is not defined for complex arrays" % name)
+
+
+def linear_cross_entropy(x, weight, target):
+    """Mean softmax cross entropy of the logits x @ weight against class numbers, without keeping the logits.
+
+    x [..., in], weight [in, classes] (as in `linear`; the transposed view of a tied embedding [classes, in] is taken as it
+    is), target: one class number per row, held as floats the way reduce_argmax returns them. Rows with a negative target
+    are left out of the mean and of every gradient; without any row left the loss is 0. A target that is no class makes the
+    loss NaN. Returns the loss, shape [1]; x and weight get gradients, to first order."""
+    _real_operands("linear_cross_entropy", x, weight, target)
+    if x.ndim() < 1 or weight.ndim() != 2 or x._shape[-1] != weight._shape[0]:
+        raise ValueError("linear_cross_entropy: x of shape %s does not multiply a weight of shape %s" % (x.shape(), weight.shape()))
+    if target.size() != x.size() // max(x._shape[-1], 1) or target._requires_grad:
+        raise ValueError("linear_cross_entropy: target holds one class number per row of x, and gets no gradient")
+    D, V = weight._shape
+    N = target.size()
+    if not (N and D and V):
+        raise ValueError("linear_cross_entropy: empty operand")
+    xs, ts = contiguous(x), contiguous(target)
+    ws, trans, ldw, _ = _gemm_operand(weight)
+    loss, lse = Array.empty([1]), Array.empty([N + 1])
+    L.call("endia_hip_linear_cross_entropy_fwd", N, D, V, xs.data_ptr(), D, trans, ws.data_ptr(), ldw, ts.data_ptr(), loss.data_ptr(),
+           lse.data_ptr())
+
+    def vjp(primals, grad, out_):
+        _first_order_only("linear_cross_entropy", grad, out_)
+        px, pw, _ = primals
+        dx = Array.empty(px._shape) if px._requires_grad else None
+        dw = Array.empty([V, D] if trans else [D, V]) if pw._requires_grad else None
+        if dx is None and dw is None:
+            return [None, None, None]
+        L.call("endia_hip_linear_cross_entropy_bwd", N, D, V, xs.data_ptr(), D, trans, ws.data_ptr(), ldw, ts.data_ptr(), lse.data_ptr(),
+               contiguous(grad).data_ptr(), dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None)
+        if dw is not None and trans:  # the gradient of a transposed view, as a transposed view
+            dw = Array([D, V], _buffer=dw._buf, _strides=[1, D])
+        return [dx, dw, None]
+
+    return _register(loss, [x, weight, target], "linear_cross_entropy", vjp)
+
+
+def _rows_in_place(a):
+    """A [batch, position, head, dim] array whose last axis is contiguous is read where it lies; others are copied."""
+    return a if a._strides[-1] == 1 or a._shape[-1] == 1 else _contiguous_copy(a)
+
+
+def _attention(name, q, k, v, table, key_lengths, causal, scale, query_offset, max_distance):
+    import ctypes
+    _real_operands(name, q, k, v, table, key_lengths)
+    if q.ndim() != 4 or k.ndim() != 4 or v.ndim() != 4:
+        raise ValueError("%s: q is [batch, queries, heads, dim], k and v are [batch, keys, heads, dim]" % name)
+    B, Q, H, D = q._shape
+    _, K, Hk, _ = k._shape
+    if v._shape != k._shape or k._shape[0] != B or k._shape[3] != D or Hk == 0 or H % Hk:
+        raise ValueError("%s: shapes %s, %s and %s do not go together" % (name, q.shape(), k.shape(), v.shape()))
+    if not (q.size() and k.size()):
+        raise ValueError("%s: empty operand" % name)
+    if table is not None and (table.ndim() != 2 or table._shape[1] != H):
+        raise ValueError("%s: the position table is [buckets, heads]" % name)
+    if key_lengths is not None and (key_lengths.size() != B or key_lengths._requires_grad):
+        raise ValueError("%s: key_lengths holds one length per batch entry, and gets no gradient" % name)
+    qs, ks, vs = _rows_in_place(q), _rows_in_place(k), _rows_in_place(v)
+    lens = contiguous(key_lengths) if key_lengths is not None else None
+    tab = contiguous(table) if table is not None else None
+    desc = L.AttentionDesc()
+    desc.B, desc.Q, desc.K, desc.H, desc.Hk, desc.D = B, Q, K, H, Hk, D
+    desc.q_strides[:], desc.k_strides[:], desc.v_strides[:] = qs._strides[:3], ks._strides[:3], vs._strides[:3]
+    desc.query_offset, desc.causal = int(query_offset), 1 if causal else 0
+    desc.scale = float(scale) if scale is not None else D ** -0.5
+    if table is not None:
+        desc.buckets, desc.max_distance, desc.both_sides = table._shape[0], int(max_distance), 0 if causal else 1
+    args = [q, k, v] + ([table] if table is not None else [])
+    out = Array.empty([B, Q, H, D])
+    lse = Array.empty([B, H, Q]) if any(a._requires_grad for a in args) else None
+    ptr = lambda a: a.data_ptr() if a is not None else None
+    L.call("endia_hip_attention_fwd", ctypes.byref(desc), qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), ptr(lens), ptr(tab), out.data_ptr(),
+           ptr(lse))
+
+    def vjp(primals, grad, out_):
+        _first_order_only(name, grad, out_)
+        grads = [Array.empty(p._shape) if p._requires_grad else None for p in primals]
+        dtable = grads[3] if table is not None else None
+        L.call("endia_hip_attention_bwd", ctypes.byref(desc), qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), ptr(lens), ptr(tab), out_.data_ptr(),
+               lse.data_ptr(), contiguous(grad).data_ptr(), ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(dtable))
+        return grads
+
+    return _register(out, args, name, vjp)
+
+
+def attention(q, k, v, key_lengths=None, causal=False, scale=None, query_offset=0):
+    """softmax(scale q k^T) v for q [batch, queries, heads, dim] over k, v [batch, keys, key_heads, dim] of another length
+    (cross attention to an encoder's states; self attention when they come from one sequence). Returns q's shape.
+
+    heads is a multiple of key_heads, each of which serves that many query heads in a row. key_lengths: one whole number
+    per batch entry, held as floats on the device; keys behind it are never read into a result, whatever they hold.
+    causal: query i sees the keys up to i + query_offset, so one new token over a cache of n tokens is query_offset = n.
+    scale defaults to dim ** -0.5. A query without any key left gives zeros, and zero gradients. dim is at most 128.
+    Views whose last axis is contiguous (slices of a fused projection) are read in place. First order only."""
+    return _attention("attention", q, k, v, None, key_lengths, causal, scale, query_offset, 0)
+
+
+def relative_attention(q, k, v, table, key_lengths=None, causal=False, scale=None, query_offset=0, max_distance=128):
+    """`attention` with a learned bias per head on the difference key position - query position: table [buckets, heads] is
+    added to the scores by bucket, and gets a gradient. Half of a side's buckets hold one difference each, the others widen
+    logarithmically up to max_distance, behind which everything shares the last one. Causal attention uses all buckets for
+    keys before the query; otherwise later keys use the second half of the (even number of) buckets."""
+    return _attention("relative_attention", q, k, v, table, key_lengths, causal, scale, query_offset, max_distance)
+
+
+# --------------------------------------------------------------------------------------------------
 # conv2d (endia/functional/spacial_ops/conv2d_op.mojo)
 # --------------------------------------------------------------------------------------------------
 def _pair(v):

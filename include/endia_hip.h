@@ -403,6 +403,57 @@ ENDIA_API int32_t endia_hip_reduce(int32_t op, int32_t ndim, const int64_t* shap
 ENDIA_API int32_t endia_hip_mse_fwd_bwd(int64_t n, const float* pred, const float* target, float* loss,
                               float* dpred);
 
+/* ---- softmax cross entropy of a linear layer, z = x W, over a large vocabulary, and its gradient, in pieces of the
+ *      vocabulary: the N x V logits are never kept. No counterpart in the reference, whose only loss is mse
+ *      (loss_ops/mse_op.mojo:17-20); this is the loss of a model that answers with one of V classes.
+ *        lse_i = log sum_j exp z_ij      loss = (1 / n) sum over kept rows i of (lse_i - z_{i, target_i})
+ *        dz_ij = (g / n) (exp(z_ij - lse_i) - [j = target_i]),   dx = dz W^T,   dW = x^T dz
+ *      x [N, D] with row stride ldx. W is D x V, element (d, v) at W[d*ldw + v], or with transW = 1 stored V x D, element
+ *      (d, v) at W[v*ldw + d] (a tied embedding). target: N class numbers held as floats; a row with a negative target is
+ *      left out: it counts neither in n nor in any gradient, whatever x holds there, and its dx is zero. n = 0 gives
+ *      loss 0. A target that is no class (NaN, or V and above) makes the loss, and the gradients that the row takes part
+ *      in, NaN.
+ *      fwd: loss is one device float; lse receives N + 1 floats (lse per row, then n), which bwd takes.
+ *      bwd: g is one device float, the cotangent of the loss. dx [N, D] and dW (in W's storage order, contiguous) are
+ *      overwritten; either may be null. */
+ENDIA_API int32_t endia_hip_linear_cross_entropy_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW,
+                                           const float* W, int64_t ldw, const float* target, float* loss, float* lse);
+ENDIA_API int32_t endia_hip_linear_cross_entropy_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW,
+                                           const float* W, int64_t ldw, const float* target, const float* lse, const float* g,
+                                           float* dx, float* dW);
+
+/* ---- attention of Q queries over K keys of another length (cross attention; self attention when they are one
+ *      sequence), with an optional learned position bias by buckets, and its gradient. No counterpart in the reference,
+ *      which would spell it in matmul, exp, sum and div nodes.
+ *        s_ij = scale q_i . k_j + table[bucket(j - (i + query_offset))][h]
+ *        p_ij = exp(s_ij) / sum_j exp(s_ij) over the keys j that are left,   o_i = sum_j p_ij v_j
+ *      q [B, Q, H, D], k and v [B, K, Hk, D]: strides in elements for the batch, position and head axes, the last axis
+ *      contiguous; H is a multiple of Hk, query head h reads key head h / (H / Hk). D <= ENDIA_ATTENTION_MAX_DIM.
+ *      key_lengths: B whole numbers held as floats, or null: keys at and behind key_lengths[b] (clamped to 0 .. K) are
+ *      left out and never take part, whatever they hold. causal: key j is left out of query i when j > i + query_offset.
+ *      A query with no key left gets o = 0, lse = -inf and no gradient.
+ *      table [buckets, H] or null. A difference of n steps has bucket n for n < e (e = half the side's buckets), then
+ *      e + floor(log(n/e) / log(max_distance/e) * (side - e)), at most side - 1. both_sides = 0: side = buckets, n counts
+ *      back from the query, later keys have n = 0. both_sides = 1: side = buckets / 2, later keys use the second half.
+ *      fwd: o [B, Q, H, D] contiguous; lse [B, H, Q] (log of the sum of exp(s)) or null.
+ *      bwd: takes the o and lse of fwd and the cotangent go [B, Q, H, D] contiguous; dq [B, Q, H, D], dk and dv
+ *      [B, K, Hk, D] (summed over the query heads that share them), dtable [buckets, H] are overwritten; any may be null. */
+#define ENDIA_ATTENTION_MAX_DIM 128
+#define ENDIA_ATTENTION_MAX_DISTANCE 2048
+typedef struct endia_hip_attention_desc {
+  int64_t B, Q, K, H, Hk, D;
+  int64_t q_strides[3], k_strides[3], v_strides[3]; /* batch, position, head */
+  int64_t query_offset;
+  float scale;
+  int32_t causal;
+  int32_t buckets, max_distance, both_sides;
+} endia_hip_attention_desc;
+ENDIA_API int32_t endia_hip_attention_fwd(const endia_hip_attention_desc* d, const float* q, const float* k, const float* v,
+                                const float* key_lengths, const float* table, float* o, float* lse);
+ENDIA_API int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* q, const float* k, const float* v,
+                                const float* key_lengths, const float* table, const float* o, const float* lse, const float* go,
+                                float* dq, float* dk, float* dv, float* dtable);
+
 /* ---- conv2d, NCHW, groups = 1: Conv2d.__call__ (spacial_ops/conv2d_op.mojo:88-196), output shape
  *      rule conv2d_op.mojo:31-85. The three gradients have no counterpart in the reference, whose
  *      Conv2d.vjp is default_vjp (conv2d_op.mojo:198-200); they are the adjoints of that forward loop.
