@@ -1,55 +1,39 @@
-// Attention of queries over keys of another length, with an optional learned position bias by buckets, and its gradient.
-// Stands beside matmul and linear (endia/functional/binary_ops/matmul_op.mojo): the products of a sequence model's layer.
+// Attention of queries over keys of another length, with an optional learned position bias by buckets, and its gradient: the
+// entry points, their checks, and the choice of kernels. Stands beside matmul and linear
+// (endia/functional/binary_ops/matmul_op.mojo): the reference would spell it in matmul, exp, sum and div nodes.
 //
 //   s_ij = scale q_i . k_j + table[bucket(j - (i + query_offset))]     masked: j >= key_lengths[b], causal j > i + query_offset
 //   p = softmax over the keys that are left (a row with none: zeros)   o = p v
-//   dv = p^T do,  dp = do v^T,  ds = p (dp - sum_j p dp),  dq = scale ds k,  dk = scale ds^T q,  dtable = sums of ds by bucket
-//
-// First form: one batch entry at a time with the score matrix in memory, products by endia_hip_sgemm.
-#include "common.h"
+//   dv = p^T do,  dp = do v^T,  ds = p (dp - do . o),  dq = scale ds k,  dk = scale ds^T q,  dtable = sums of ds by bucket
+#include "attention.h"
 
 #include <math.h>
 
 using namespace endia;
+using namespace attention;
 
 namespace {
 
-constexpr int TPB = 256;
-constexpr int kMaxSide = 128;  // buckets of one side
-
+// Pooled memory for the time of one call: work on the one stream is ordered, so it can go back at once.
 struct Scratch {
   void* p = nullptr;
-  int32_t get(int64_t bytes) { return endia_hip_malloc(bytes, &p); }
+  int64_t used = 0;
   ~Scratch() {
     if (p) endia_hip_free(p);
   }
-  float* f() const { return static_cast<float*>(p); }
-};
-
-// bucket of n steps: n itself below `exact`, then the largest i with start[i] <= n
-struct Buckets {
-  int side, exact, both;
-  int start[kMaxSide];
-};
-
-__device__ __forceinline__ int bucket_of(const Buckets& t, int64_t rel) {
-  int base = 0;
-  int64_t n = -rel;
-  if (t.both) {
-    if (rel > 0) {
-      base = t.side;
-      n = rel;
-    }
-  } else if (n < 0) {
-    n = 0;
+  int64_t want(int64_t bytes) {  // offset of a piece
+    const int64_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    return at;
   }
-  if (n < t.exact) return base + (int)n;
-  int i = t.exact;
-  while (i + 1 < t.side && t.start[i + 1] <= n) ++i;
-  return base + i;
-}
+  int32_t get() { return endia_hip_malloc(used, &p); }
+  template <typename T>
+  T* at(int64_t offset) const {
+    return reinterpret_cast<T*>(static_cast<char*>(p) + offset);
+  }
+};
 
-int32_t make_buckets(const endia_hip_attention_desc* d, Buckets* t) {
+void make_buckets(const endia_hip_attention_desc* d, Buckets* t) {
   t->both = d->both_sides;
   t->side = d->both_sides ? d->buckets / 2 : d->buckets;
   t->exact = t->side / 2;
@@ -61,90 +45,7 @@ int32_t make_buckets(const endia_hip_attention_desc* d, Buckets* t) {
     const int far = t->exact + (int)floor(log((double)n / t->exact) / log((double)d->max_distance / t->exact) * steps + 1e-9);
     while (i < t->side && i <= far) t->start[i++] = n;
   }
-  return ENDIA_HIP_OK;
-}
-
-__device__ __forceinline__ float block_reduce(float v, float* red, bool maximum) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const float u = __shfl_xor(v, o, 64);
-    v = maximum ? fmaxf(v, u) : v + u;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < TPB / 64; ++w) v = maximum ? fmaxf(v, red[w]) : v + red[w];
-  return v;
-}
-
-__device__ __forceinline__ int64_t key_count(const float* lengths, int64_t b, int64_t K) {
-  if (!lengths) return K;
-  const float n = lengths[b];
-  return n > 0.f ? (n < (float)K ? (int64_t)n : K) : 0;
-}
-
-// k or v of one batch entry as [Hk, K, D], zeros behind the entry's length
-__global__ __launch_bounds__(TPB) void clean_kernel(const float* __restrict__ x, int64_t sp, int64_t sh, const float* __restrict__ lengths, int64_t b,
-                                                    int64_t K, int64_t D, float* __restrict__ out) {
-  const int64_t j = blockIdx.x, h = blockIdx.y, n = key_count(lengths, b, K);
-  for (int64_t d = threadIdx.x; d < D; d += TPB) out[(h * K + j) * D + d] = j < n ? x[j * sp + h * sh + d] : 0.f;
-}
-
-__global__ __launch_bounds__(TPB) void softmax_kernel(float* __restrict__ s, int64_t Q, int64_t K, int64_t b, int64_t H, const float* __restrict__ lengths,
-                                                      float scale, int causal, int64_t off, const float* __restrict__ table, Buckets bk,
-                                                      float* __restrict__ lse) {
-  __shared__ float red[TPB / 64];
-  const int64_t i = blockIdx.x, h = blockIdx.y;
-  int64_t n = key_count(lengths, b, K);
-  if (causal && i + off + 1 < n) n = i + off + 1 > 0 ? i + off + 1 : 0;
-  float* row = s + (h * Q + i) * K;
-  float top = -INFINITY;
-  for (int64_t j = threadIdx.x; j < n; j += TPB) {
-    float t = row[j] * scale;
-    if (table) t += table[bucket_of(bk, j - (i + off)) * H + h];
-    row[j] = t;
-    top = fmaxf(top, t);
-  }
-  top = block_reduce(top, red, true);
-  float sum = 0.f;
-  for (int64_t j = threadIdx.x; j < n; j += TPB) sum += expf(row[j] - top);
-  sum = block_reduce(sum, red, false);
-  const float e = top + logf(sum);
-  for (int64_t j = threadIdx.x; j < K; j += TPB) row[j] = j < n ? expf(row[j] - e) : 0.f;
-  if (threadIdx.x == 0 && lse) lse[(b * H + h) * Q + i] = n ? e : -INFINITY;
-}
-
-__global__ __launch_bounds__(TPB) void ds_kernel(const float* __restrict__ p, float* __restrict__ dp, int64_t K) {
-  __shared__ float red[TPB / 64];
-  const int64_t r = blockIdx.x * K;
-  float sum = 0.f;
-  for (int64_t j = threadIdx.x; j < K; j += TPB) sum += p[r + j] * dp[r + j];
-  sum = block_reduce(sum, red, false);
-  for (int64_t j = threadIdx.x; j < K; j += TPB) dp[r + j] = p[r + j] * (dp[r + j] - sum);
-}
-
-// dtable[bucket, h] (+)= the sum of ds over the pairs of that bucket; one group per (bucket, h)
-__global__ __launch_bounds__(TPB) void table_grad_kernel(const float* __restrict__ ds, int64_t Q, int64_t K, int64_t H, int64_t off, Buckets bk,
-                                                         float* __restrict__ dtable, int first) {
-  __shared__ double red[TPB];
-  const int b = blockIdx.x;
-  const int64_t h = blockIdx.y;
-  double sum = 0.0;
-  for (int64_t j = threadIdx.x; j < Q * K; j += TPB)
-    if (bucket_of(bk, j % K - (j / K + off)) == b) sum += (double)ds[h * Q * K + j];
-  red[threadIdx.x] = sum;
-  __syncthreads();
-  for (int s = TPB / 2; s; s >>= 1) {
-    if (threadIdx.x < s) red[threadIdx.x] += red[threadIdx.x + s];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) dtable[b * H + h] = (first ? 0.f : dtable[b * H + h]) + (float)red[0];
-}
-
-__global__ __launch_bounds__(TPB) void scale_kernel(float* __restrict__ x, int64_t n, float c) {
-  const int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x;
-  if (i < n) x[i] *= c;
+  t->near = t->start[t->side - 1];  // (max_distance itself is in the last bucket, so all starts are set)
 }
 
 int32_t check(const char* who, const endia_hip_attention_desc* d, const float* q, const float* k, const float* v, const float* table) {
@@ -154,9 +55,10 @@ int32_t check(const char* who, const endia_hip_attention_desc* d, const float* q
   ENDIA_CHECK_ARG(d->Q < (1ll << 24) && d->K <= (1ll << 24), "%s: more than 2^24 positions (lengths are held in fp32)", who);
   ENDIA_CHECK_ARG(d->query_offset > -(1ll << 30) && d->query_offset < (1ll << 30), "%s: query_offset out of range", who);
   ENDIA_CHECK_ARG(isfinite(d->scale), "%s: scale must be finite", who);
-  if (d->D > ENDIA_ATTENTION_MAX_DIM || d->B * d->H > 65535)
-    return fail(ENDIA_HIP_ERR_UNSUPPORTED, "%s: head dimension %lld above %d, or more than 65535 heads over the batch", who, (long long)d->D,
-                ENDIA_ATTENTION_MAX_DIM);
+  if (d->D > ENDIA_ATTENTION_MAX_DIM || d->B > 65535 || d->H > 32767 || d->B * d->H > 65535 || d->B * d->H * ceil_div64(d->Q, 32) >= (1ll << 31) ||
+      d->B * d->Hk * ceil_div64(d->K, 32) >= (1ll << 31))
+    return fail(ENDIA_HIP_ERR_UNSUPPORTED, "%s: head dimension %lld above %d, more than 65535 heads over the batch, or too many rows", who,
+                (long long)d->D, ENDIA_ATTENTION_MAX_DIM);
   if (table) {
     const int side = d->both_sides ? d->buckets / 2 : d->buckets;
     ENDIA_CHECK_ARG(side >= 2 && (!d->both_sides || d->buckets % 2 == 0) && d->max_distance > side / 2,
@@ -166,6 +68,39 @@ int32_t check(const char* who, const endia_hip_attention_desc* d, const float* q
                   ENDIA_ATTENTION_MAX_DISTANCE);
   }
   return ENDIA_HIP_OK;
+}
+
+bool on16(const float* p, const int64_t* strides) {
+  bool ok = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+  for (int i = 0; strides && i < 3; ++i) ok = ok && strides[i] % 4 == 0;
+  return ok;
+}
+
+Args make_args(const endia_hip_attention_desc* d, const float* q, const float* k, const float* v, const float* lengths, const float* table) {
+  Args a = {};
+  a.B = d->B; a.Q = d->Q; a.K = d->K; a.H = d->H; a.Hk = d->Hk; a.D = d->D; a.G = d->H / d->Hk;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = d->q_strides[i];
+    a.ks[i] = d->k_strides[i];
+    a.vs[i] = d->v_strides[i];
+  }
+  a.off = d->query_offset;
+  a.scale = d->scale;
+  a.causal = d->causal ? 1 : 0;
+  a.q = q; a.k = k; a.v = v; a.lengths = lengths; a.table = table;
+  a.vec = d->D % 4 == 0 && on16(q, d->q_strides) && on16(k, d->k_strides) && on16(v, d->v_strides);
+  a.splits = 1;
+  if (table) make_buckets(d, &a.bk);
+  return a;
+}
+
+int padded_dim(int64_t D) { return (int)((D + 31) / 32 * 32); }
+
+// Into how many parts a walk of `steps` is cut so that `groups` work-groups become about `want`; a part has at least `least` steps.
+int parts(int64_t groups, int64_t want, int64_t steps, int64_t least) {
+  int64_t p = (want + groups - 1) / groups;
+  if (p > steps / least) p = steps / least;
+  return (int)(p < 1 ? 1 : p > 256 ? 256 : p);
 }
 
 }  // namespace
@@ -179,30 +114,40 @@ int32_t endia_hip_attention_fwd(const endia_hip_attention_desc* d, const float* 
   ENDIA_CHECK_ARG(o, "endia_hip_attention_fwd: null pointer");
   ENDIA_REQUIRE_INIT();
   hipStream_t st = ctx().stream;
-  const int64_t B = d->B, Q = d->Q, K = d->K, H = d->H, Hk = d->Hk, D = d->D, G = H / Hk;
-  Buckets bk = {};
-  if (table) make_buckets(d, &bk);
-  Scratch s, kc, vc;
-  if ((rc = s.get(4 * H * Q * K)) || (rc = kc.get(4 * Hk * K * D)) || (rc = vc.get(4 * Hk * K * D))) return rc;
-  for (int64_t b = 0; b < B; ++b) {
-    hipLaunchKernelGGL(clean_kernel, dim3((unsigned)K, (unsigned)Hk), dim3(TPB), 0, st, k + b * d->k_strides[0], d->k_strides[1], d->k_strides[2],
-                       key_lengths, b, K, D, kc.f());
-    hipLaunchKernelGGL(clean_kernel, dim3((unsigned)K, (unsigned)Hk), dim3(TPB), 0, st, v + b * d->v_strides[0], d->v_strides[1], d->v_strides[2],
-                       key_lengths, b, K, D, vc.f());
-    for (int64_t c = 0; c < Hk; ++c)
-      if ((rc = endia_hip_sgemm(0, 1, Q, K, D, q + b * d->q_strides[0] + c * G * d->q_strides[2], d->q_strides[1], kc.f() + c * K * D, D,
-                                s.f() + c * G * Q * K, K, G, d->q_strides[2], 0, Q * K, ENDIA_EPI_NONE, ENDIA_OP_IDENTITY, nullptr, nullptr,
-                                nullptr)))
-        return rc;
-    hipLaunchKernelGGL(softmax_kernel, dim3((unsigned)Q, (unsigned)H), dim3(TPB), 0, st, s.f(), Q, K, b, H, key_lengths, d->scale, d->causal,
-                       d->query_offset, table, bk, lse);
-    for (int64_t h = 0; h < H; ++h)
-      if ((rc = endia_hip_sgemm(0, 0, Q, D, K, s.f() + h * Q * K, K, vc.f() + h / G * K * D, D, o + b * Q * H * D + h * D, H * D, 1, 0, 0, 0,
-                                ENDIA_EPI_NONE, ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr)))
-        return rc;
+  Args a = make_args(d, q, k, v, key_lengths, table);
+  a.vec = a.vec && on16(o, nullptr);
+  a.o = o;
+  a.lse = lse;
+  const int64_t rows = a.G * a.Q, cus = ctx().cu_count;
+  Scratch w;
+  if (rows <= 16) {
+    int R = rows == 1 ? 1 : rows == 2 ? 2 : 4;
+    while (table && R > 1 && R * (2 * a.bk.near + 1) * 4 > 32 * 1024) R /= 2;  // a bias table per head of the rows
+    const int64_t step = (a.D <= 32 ? 32 : a.D <= 64 ? 16 : 8) * (R <= 2 ? 4 : 2);
+    a.splits = parts(ceil_div64(rows, R) * a.B * a.Hk, 4 * cus, ceil_div64(a.K, step), 2);
+    if (a.splits > 1) {
+      const int64_t n = a.B * a.H * a.Q * a.splits, part = w.want(4 * n * a.D), ml = w.want(8 * n);
+      if ((rc = w.get())) return rc;
+      a.part = w.at<float>(part);
+      a.part_ml = w.at<float>(ml);
+    }
+    return launch_rows(a, R, st);
   }
-  ENDIA_LAUNCH_CHECK();
-  return ENDIA_HIP_OK;
+  const int DP = padded_dim(a.D);
+  const int64_t tiles = ceil_div64(a.K, kTile), images = a.B * a.Hk * tiles * DP * 128;
+  a.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, 2 * cus, tiles, 4);
+  const int64_t n = a.splits > 1 ? a.B * a.H * a.Q * a.splits : 0;
+  const int64_t kr = w.want(images), vc = w.want(images), ks = w.want(4 * a.B * a.Hk * tiles), vs = w.want(4 * a.B * a.Hk * tiles),
+                part = w.want(4 * n * a.D), ml = w.want(8 * n);
+  if ((rc = w.get())) return rc;
+  a.k_rows = w.at<char>(kr);
+  a.v_cols = w.at<char>(vc);
+  a.k_shift = w.at<int>(ks);
+  a.v_shift = w.at<int>(vs);
+  a.part = w.at<float>(part);
+  a.part_ml = w.at<float>(ml);
+  if ((rc = launch_tiles(a, DP, false, st))) return rc;
+  return launch_forward(a, DP, st);
 }
 
 int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* q, const float* k, const float* v, const float* key_lengths,
@@ -215,48 +160,39 @@ int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* 
   ENDIA_CHECK_ARG(!dtable || table, "endia_hip_attention_bwd: dtable without a table");
   ENDIA_REQUIRE_INIT();
   hipStream_t st = ctx().stream;
-  const int64_t B = d->B, Q = d->Q, K = d->K, H = d->H, Hk = d->Hk, D = d->D, G = H / Hk;
-  Buckets bk = {};
-  if (table) make_buckets(d, &bk);
-  Scratch s, ds, kc, vc;
-  if ((rc = s.get(4 * H * Q * K)) || (rc = ds.get(4 * H * Q * K)) || (rc = kc.get(4 * Hk * K * D)) || (rc = vc.get(4 * Hk * K * D))) return rc;
-  for (int64_t b = 0; b < B; ++b) {
-    hipLaunchKernelGGL(clean_kernel, dim3((unsigned)K, (unsigned)Hk), dim3(TPB), 0, st, k + b * d->k_strides[0], d->k_strides[1], d->k_strides[2],
-                       key_lengths, b, K, D, kc.f());
-    hipLaunchKernelGGL(clean_kernel, dim3((unsigned)K, (unsigned)Hk), dim3(TPB), 0, st, v + b * d->v_strides[0], d->v_strides[1], d->v_strides[2],
-                       key_lengths, b, K, D, vc.f());
-    const float* qb = q + b * d->q_strides[0];
-    const float* gb = go + b * Q * H * D;
-    for (int64_t c = 0; c < Hk; ++c) {
-      if ((rc = endia_hip_sgemm(0, 1, Q, K, D, qb + c * G * d->q_strides[2], d->q_strides[1], kc.f() + c * K * D, D, s.f() + c * G * Q * K, K, G,
-                                d->q_strides[2], 0, Q * K, ENDIA_EPI_NONE, ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr)) ||
-          (rc = endia_hip_sgemm(0, 1, Q, K, D, gb + c * G * D, H * D, vc.f() + c * K * D, D, ds.f() + c * G * Q * K, K, G, D, 0, Q * K,
-                                ENDIA_EPI_NONE, ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr)))
-        return rc;
-    }
-    hipLaunchKernelGGL(softmax_kernel, dim3((unsigned)Q, (unsigned)H), dim3(TPB), 0, st, s.f(), Q, K, b, H, key_lengths, d->scale, d->causal,
-                       d->query_offset, table, bk, nullptr);
-    hipLaunchKernelGGL(ds_kernel, dim3((unsigned)(H * Q)), dim3(TPB), 0, st, s.f(), ds.f(), K);
-    if (dtable)
-      hipLaunchKernelGGL(table_grad_kernel, dim3((unsigned)d->buckets, (unsigned)H), dim3(TPB), 0, st, ds.f(), Q, K, H, d->query_offset, bk, dtable,
-                         b == 0 ? 1 : 0);
-    for (int64_t h = 0; h < H; ++h) {
-      const int64_t c = h / G, at = h * Q * K;
-      const int32_t more = h % G ? ENDIA_EPI_NONE | ENDIA_GEMM_ACCUMULATE : ENDIA_EPI_NONE;
-      if (dv && (rc = endia_hip_sgemm(1, 0, K, D, Q, s.f() + at, K, gb + h * D, H * D, dv + b * K * Hk * D + c * D, Hk * D, 1, 0, 0, 0, more,
-                                      ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr)))
-        return rc;
-      if (dk && (rc = endia_hip_sgemm(1, 0, K, D, Q, ds.f() + at, K, qb + h * d->q_strides[2], d->q_strides[1], dk + b * K * Hk * D + c * D, Hk * D,
-                                      1, 0, 0, 0, more, ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr)))
-        return rc;
-      if (dq && (rc = endia_hip_sgemm(0, 0, Q, D, K, ds.f() + at, K, kc.f() + c * K * D, D, dq + b * Q * H * D + h * D, H * D, 1, 0, 0, 0,
-                                      ENDIA_EPI_NONE, ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr)))
-        return rc;
-    }
+  Args a = make_args(d, q, k, v, key_lengths, table);
+  a.vec = a.vec && on16(o, nullptr) && on16(go, nullptr) && on16(dq, nullptr) && on16(dk, nullptr) && on16(dv, nullptr);
+  a.out = o;
+  a.lse = const_cast<float*>(lse);
+  a.go = go;
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  const int DP = padded_dim(a.D);
+  const int64_t cus = ctx().cu_count, kt = ceil_div64(a.K, kTile), qt = ceil_div64(a.Q, kTile);
+  const int64_t kn = a.B * a.Hk * kt, qn = a.B * a.H * qt, image = DP * 128;
+  const bool queries = dq || dtable, keys = dk || dv;
+  Args aq = a, ak = a;
+  aq.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, 2 * cus, kt, 4);
+  ak.splits = parts(ceil_div64(a.K, 128) * a.Hk * a.B, 2 * cus, a.G * qt, 4);
+  Scratch w;
+  const int64_t kr = w.want(kn * image), kc = w.want(kn * image), vr = w.want(kn * image), qr = w.want(qn * image), qc = w.want(qn * image),
+                gr = w.want(qn * image), gc = w.want(qn * image), ksh = w.want(4 * kn), vsh = w.want(4 * kn), qsh = w.want(4 * qn),
+                gsh = w.want(4 * qn), meta = w.want(256 * qn);
+  const int64_t part_q = aq.splits > 1 ? 4 * aq.splits * a.B * a.Q * a.H * a.D : 0, part_k = ak.splits > 1 ? 8 * ak.splits * a.B * a.K * a.Hk * a.D : 0;
+  const int64_t part = w.want(part_q > part_k ? part_q : part_k);  // (one after the other on the stream)
+  const int64_t table_part = w.want(dtable ? table_groups(aq) * (2 * a.bk.near + 1) * 4 : 0);
+  if ((rc = w.get())) return rc;
+  for (Args* x : {&a, &aq, &ak}) {
+    x->k_rows = w.at<char>(kr); x->k_cols = w.at<char>(kc); x->v_rows = w.at<char>(vr); x->q_rows = w.at<char>(qr);
+    x->q_cols = w.at<char>(qc); x->g_rows = w.at<char>(gr); x->g_cols = w.at<char>(gc);
+    x->k_shift = w.at<int>(ksh); x->v_shift = w.at<int>(vsh); x->q_shift = w.at<int>(qsh); x->g_shift = w.at<int>(gsh);
+    x->meta = w.at<float>(meta);
+    x->part = w.at<float>(part);
+    x->part_table = dtable ? w.at<float>(table_part) : nullptr;
   }
-  if (dq) hipLaunchKernelGGL(scale_kernel, dim3((unsigned)ceil_div64(B * Q * H * D, TPB)), dim3(TPB), 0, st, dq, B * Q * H * D, d->scale);
-  if (dk) hipLaunchKernelGGL(scale_kernel, dim3((unsigned)ceil_div64(B * K * Hk * D, TPB)), dim3(TPB), 0, st, dk, B * K * Hk * D, d->scale);
-  ENDIA_LAUNCH_CHECK();
+  if ((rc = launch_tiles(a, DP, true, st))) return rc;
+  if (queries && (rc = launch_dq(aq, DP, st))) return rc;
+  if (dtable && (rc = launch_table_grad(aq, dtable, st))) return rc;
+  if (keys && (rc = launch_dkv(ak, DP, st))) return rc;
   return ENDIA_HIP_OK;
 }
 

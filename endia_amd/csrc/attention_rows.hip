@@ -1,0 +1,202 @@
+// Attention for few queries per key head: the serving form, one or a few new tokens over a long cache. Bound: HBM, k and v are
+// read once.
+//
+// A work-group of four waves takes R rows (query i of query head g, numbered g Q + i, of the G heads that share a key head) and
+// one part of the keys; a key's row is read by LPK lanes, 16 bytes each, so a wave has 64 / LPK keys in hand at a time, UNROLL of
+// them in flight per lane group. Scores are sums over a lane group; every lane group keeps its own running maximum, sum and
+// output (a wave reads neither LDS nor other lanes' state per key), and the groups and waves meet once at the end. With few
+// sequences the keys are cut into parts, and combine_kernel joins the parts' results.
+#include "attention.h"
+
+namespace attention {
+
+namespace {
+
+constexpr int TPB = 256;
+
+// A group's maximum may still be -inf (no key seen): nothing to carry over then.
+__device__ __forceinline__ float carry(float m, float now) { return m == -INFINITY ? 0.f : exp2_fast(m - now); }
+
+template <int LPK, int R, bool VEC>
+__global__ __launch_bounds__(TPB) void rows_kernel(Args a) {
+  constexpr int KPW = 64 / LPK, UNROLL = R <= 2 ? 4 : 2, DP = LPK * 4;
+  constexpr int GROUPS = 4 * KPW;  // lane groups of the work-group
+  __shared__ float lds_m[R][GROUPS], lds_l[R][GROUPS];
+  __shared__ __attribute__((aligned(16))) float lds_o[R][GROUPS][DP];
+  extern __shared__ float bias_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = lane / LPK, dl = lane % LPK;
+  const int64_t b = blockIdx.z / (uint32_t)a.Hk, kh = blockIdx.z % (uint32_t)a.Hk;
+  const int64_t rows = a.G * a.Q, r0 = (int64_t)blockIdx.x * R;
+  const int D = (int)a.D;
+
+  float4 q[R];
+  int64_t place[R];   // position of the row's query
+  int limit[R];       // keys the row may see
+  const int n = key_count(a, b);
+  int most = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = r0 + r;
+    const bool in = row < rows;
+    const uint32_t g = in ? (uint32_t)row / (uint32_t)a.Q : 0, i = in ? (uint32_t)row % (uint32_t)a.Q : 0;
+    q[r] = load4<VEC>(a.q + b * a.qs[0] + i * a.qs[1] + (kh * a.G + g) * a.qs[2], 4 * dl, D, in);
+    const float c = a.scale * kLog2e;
+    q[r].x *= c; q[r].y *= c; q[r].z *= c; q[r].w *= c;
+    place[r] = i + a.off;
+    int64_t see = n;
+    if (a.causal && place[r] + 1 < see) see = place[r] + 1;
+    limit[r] = in && see > 0 ? (int)see : 0;
+    most = max(most, limit[r]);
+  }
+  const bool bias = a.table != nullptr;
+  const int near = a.bk.near, span = 2 * near + 1;
+  if (bias) {  // the heads of the work-group's rows, one table after the other (all rows of one head: one)
+    const int64_t g0 = r0 / a.Q, g1 = min(r0 + R - 1, rows - 1) / a.Q;
+    for (int64_t g = g0; g <= g1; ++g) load_bias(a, (int)(kh * a.G + g), bias_lds + (g - g0) * span, tid, TPB);
+    __syncthreads();
+  }
+  float m[R], l[R];
+  float4 o[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // this part's keys: whole steps of GROUPS * UNROLL
+  constexpr int STEP = GROUPS * UNROLL;
+  const int steps = (most + STEP - 1) / STEP, per = (steps + a.splits - 1) / a.splits;
+  const int first = blockIdx.y * per * STEP, last = min(most, first + per * STEP);
+  const float* kb = a.k + b * a.ks[0] + kh * a.ks[2];
+  const float* vb = a.v + b * a.vs[0] + kh * a.vs[2];
+  for (int j0 = first + wave * KPW + sub; j0 < last; j0 += STEP) {
+    float4 kf[UNROLL], vf[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int j = min(j0 + u * GROUPS, last - 1);
+      kf[u] = load4<VEC>(kb + (int64_t)j * a.ks[1], 4 * dl, D, true);
+      vf[u] = load4<VEC>(vb + (int64_t)j * a.vs[1], 4 * dl, D, true);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float t[UNROLL], top = m[r];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        float d = (q[r].x * kf[u].x + q[r].y * kf[u].y) + (q[r].z * kf[u].z + q[r].w * kf[u].w);
+#pragma unroll
+        for (int w = LPK / 2; w; w >>= 1) d += __shfl_xor(d, w, 64);
+        const int j = j0 + u * GROUPS;
+        if (bias) {
+          const int64_t g = (r0 + r) / a.Q - r0 / a.Q;
+          const int64_t rel = (int64_t)j - place[r];
+          const int at = rel < -near ? 0 : (rel > near ? 2 * near : (int)rel + near);
+          d += (r0 + r < rows) ? bias_lds[g * span + at] : 0.f;
+        }
+        t[u] = j < limit[r] && j < last ? d : -INFINITY;
+        top = fmaxf(top, t[u]);
+      }
+      if (top == -INFINITY) continue;
+      const float keep = carry(m[r], top);
+      m[r] = top;
+      l[r] *= keep;
+      o[r].x *= keep; o[r].y *= keep; o[r].z *= keep; o[r].w *= keep;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (t[u] == -INFINITY) continue;  // a key that is left out adds nothing, whatever its row holds
+        const float p = exp2_fast(t[u] - top);
+        l[r] += p;
+        o[r].x += p * vf[u].x; o[r].y += p * vf[u].y; o[r].z += p * vf[u].z; o[r].w += p * vf[u].w;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int g = wave * KPW + sub;
+    if (dl == 0) {
+      lds_m[r][g] = m[r];
+      lds_l[r][g] = l[r];
+    }
+    *reinterpret_cast<float4*>(&lds_o[r][g][4 * dl]) = o[r];
+  }
+  __syncthreads();
+  // thread t: element t % DP of row t / DP (+ more rows)
+  for (int at = tid; at < R * DP; at += TPB) {
+    const int r = at / DP, d = at % DP;
+    const int64_t row = r0 + r;
+    if (row >= rows) continue;
+    float top = -INFINITY;
+    for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, lds_m[r][g]);
+    float sum = 0.f, out = 0.f;
+    if (top > -INFINITY)
+      for (int g = 0; g < GROUPS; ++g) {
+        const float w = carry(lds_m[r][g], top);
+        sum += w * lds_l[r][g];
+        out += w * lds_o[r][g][d];
+      }
+    const int64_t h = kh * a.G + row / a.Q, i = row % a.Q;
+    if (a.splits == 1) {
+      if (d < D) a.o[((b * a.Q + i) * a.H + h) * D + d] = sum != 0.f ? out / sum : 0.f;
+      if (d == 0 && a.lse) a.lse[(b * a.H + h) * a.Q + i] = sum != 0.f ? (top + log2_fast(sum)) * kLn2 : -INFINITY;
+    } else {
+      const int64_t part = ((b * a.H + h) * a.Q + i) * a.splits + blockIdx.y;
+      if (d < D) a.part[part * D + d] = out;
+      if (d == 0) {
+        a.part_ml[2 * part] = top;
+        a.part_ml[2 * part + 1] = sum;
+      }
+    }
+  }
+}
+
+// One work-group per row: joins the parts' outputs, each relative to its part's maximum.
+__global__ __launch_bounds__(128) void combine_kernel(Args a) {
+  const int64_t row = blockIdx.x;  // (b H + h) Q + i
+  const int64_t i = row % a.Q, h = row / a.Q % a.H, b = row / a.Q / a.H;
+  const float* ml = a.part_ml + 2 * row * a.splits;
+  float top = -INFINITY, sum = 0.f;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
+  const int d = threadIdx.x;
+  float out = 0.f;
+  if (top > -INFINITY)
+    for (int s = 0; s < a.splits; ++s) {
+      const float w = carry(ml[2 * s], top);
+      sum += w * ml[2 * s + 1];
+      if (d < a.D) out += w * a.part[(row * a.splits + s) * a.D + d];
+    }
+  if (d < a.D) a.o[((b * a.Q + i) * a.H + h) * a.D + d] = sum != 0.f ? out / sum : 0.f;
+  if (d == 0 && a.lse) a.lse[row] = sum != 0.f ? (top + log2_fast(sum)) * kLn2 : -INFINITY;
+}
+
+template <int LPK, int R>
+int32_t launch(const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div64(a.G * a.Q, R), (unsigned)a.splits, (unsigned)(a.B * a.Hk));
+  size_t lds = 0;
+  if (a.table) {  // heads that R consecutive rows can touch
+    const int64_t heads = a.Q >= R ? 2 : ceil_div64(R, a.Q) + 1;
+    lds = (size_t)((heads < a.G ? heads : a.G) * (2 * a.bk.near + 1)) * 4;
+  }
+  if (a.vec) hipLaunchKernelGGL((rows_kernel<LPK, R, true>), grid, dim3(TPB), lds, s, a);
+  else hipLaunchKernelGGL((rows_kernel<LPK, R, false>), grid, dim3(TPB), lds, s, a);
+  ENDIA_LAUNCH_CHECK();
+  return ENDIA_HIP_OK;
+}
+
+template <int LPK>
+int32_t launch(const Args& a, int R, hipStream_t s) {
+  return R == 1 ? launch<LPK, 1>(a, s) : R == 2 ? launch<LPK, 2>(a, s) : launch<LPK, 4>(a, s);
+}
+
+}  // namespace
+
+int32_t launch_rows(const Args& a, int R, hipStream_t s) {
+  int32_t rc = a.D <= 32 ? launch<8>(a, R, s) : a.D <= 64 ? launch<16>(a, R, s) : launch<32>(a, R, s);
+  return rc || a.splits == 1 ? rc : launch_combine(a, s);
+}
+
+int32_t launch_combine(const Args& a, hipStream_t s) {
+  hipLaunchKernelGGL(combine_kernel, dim3((unsigned)(a.B * a.H * a.Q)), dim3(128), 0, s, a);
+  ENDIA_LAUNCH_CHECK();
+  return ENDIA_HIP_OK;
+}
+
+}  // namespace attention
