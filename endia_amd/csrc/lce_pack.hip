@@ -1,0 +1,136 @@
+// Operands of the linear cross entropy as panels of fp16 pairs (linear_cross_entropy.h), scaled by one power of two per row.
+// Bound: HBM; 4 bytes read (8 where the scale takes a walk of its own and the source is larger than the last-level cache) and 4
+// written per element.
+#include "linear_cross_entropy.h"
+
+namespace lce {
+
+namespace {
+
+using namespace pairs;
+constexpr int TPB = 256;
+
+__device__ __forceinline__ void store_chunk(char* line, int row, int chunk, const float (&v)[8], int shift) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = scaled(v[e], shift);
+  half8 hi, lo;
+  split8(y, hi, lo);
+  *reinterpret_cast<half8*>(line + ((chunk ^ (row & 7)) << 4)) = hi;
+  *reinterpret_cast<half8*>(line + (((4 + chunk) ^ (row & 7)) << 4)) = lo;
+}
+
+// Source rows contiguous along k: one wave per row, the row twice (the second time from cache).
+template <bool VEC>
+__global__ __launch_bounds__(TPB) void pack_rows_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, const float* __restrict__ left_out,
+                                                        char* __restrict__ panels, float* __restrict__ amax_out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const bool skip = left_out && left_out[row] < 0.f;
+  const float* r = x + row * ld;
+  float amax = 0.f;
+  auto load8 = [&](int64_t k0, float (&v)[8]) {
+    if (VEC) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int64_t at = k0 + 4 * j;
+        const float4 f = at < k ? *reinterpret_cast<const float4*>(r + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = k0 + e < k ? r[k0 + e] : 0.f;
+    }
+  };
+  if (!skip)
+    for (int64_t k0 = lane * 8; k0 < k; k0 += 512) {
+      float v[8];
+      load8(k0, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(v[e]));
+    }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+  if (lane == 0) amax_out[row] = amax;
+  const int shift = shift_of(amax);
+  const int64_t kblocks = (k + kBlock - 1) / kBlock;
+  for (int64_t k0 = lane * 8; k0 < kblocks * kBlock; k0 += 512) {
+    float v[8] = {};
+    if (!skip) load8(k0, v);
+    store_chunk(line_at(panels, row, k0 / kBlock, kblocks), (int)(row & 7), (int)(k0 % kBlock / 8), v, shift);
+  }
+}
+
+// Source [k][row]: the largest of each column first (a maximum does not depend on the order, so atomics will do) ...
+__global__ __launch_bounds__(TPB) void zero_kernel(float* __restrict__ x, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x;
+  if (i < n) x[i] = 0.f;
+}
+
+__global__ __launch_bounds__(TPB) void col_amax_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, int64_t per,
+                                                       const float* __restrict__ left_out, float* __restrict__ amax) {
+  const int64_t r = (int64_t)blockIdx.x * TPB + threadIdx.x, k0 = (int64_t)blockIdx.y * per, k1 = k0 + per < k ? k0 + per : k;
+  if (r >= rows) return;
+  float m = 0.f;
+#pragma unroll 8
+  for (int64_t i = k0; i < k1; ++i) {
+    const float v = finite_abs(x[i * ld + r]);
+    m = fmaxf(m, left_out && left_out[i] < 0.f ? 0.f : v);
+  }
+  atomicMax(reinterpret_cast<unsigned*>(amax) + r, __float_as_uint(m));
+}
+
+// ... then blocks of 32 k x 128 rows through LDS.
+__global__ __launch_bounds__(TPB) void pack_cols_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, const float* __restrict__ left_out,
+                                                        char* __restrict__ panels, const float* __restrict__ amax) {
+  __shared__ float t[kBlock][129];
+  const int tid = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * 128, kb = blockIdx.y, kblocks = (k + kBlock - 1) / kBlock;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int kk = i * 2 + (tid >> 7), rr = tid & 127;
+    const int64_t kg = kb * kBlock + kk, r = r0 + rr;
+    const bool in = kg < k && r < rows && !(left_out && left_out[kg] < 0.f);
+    t[kk][rr] = in ? x[kg * ld + r] : 0.f;
+  }
+  __syncthreads();
+  const int rr = tid & 127;
+  const int64_t row = r0 + rr;
+  if (row >= rows) return;
+  const int shift = shift_of(amax[row]);
+  char* line = line_at(panels, row, kb, kblocks);
+#pragma unroll
+  for (int c = tid >> 7; c < 4; c += 2) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = t[c * 8 + e][rr];
+    store_chunk(line, (int)(row & 7), c, v, shift);
+  }
+}
+
+}  // namespace
+
+int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax, hipStream_t s) {
+  if (!transposed) {
+    const bool vec = k % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    const dim3 grid((unsigned)ceil_div64(rows, 4));
+    if (vec) hipLaunchKernelGGL(pack_rows_kernel<true>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax);
+    else hipLaunchKernelGGL(pack_rows_kernel<false>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax);
+    ENDIA_LAUNCH_CHECK();
+    return ENDIA_HIP_OK;
+  }
+  hipLaunchKernelGGL(zero_kernel, dim3((unsigned)ceil_div64(rows, TPB)), dim3(TPB), 0, s, amax, rows);
+  const int64_t groups = ceil_div64(rows, TPB);
+  int64_t cuts = ceil_div64(4096, groups);
+  if (cuts > ceil_div64(k, 16)) cuts = ceil_div64(k, 16);
+  if (cuts > 65535) cuts = 65535;
+  const int64_t per = ceil_div64(k, cuts);
+  hipLaunchKernelGGL(col_amax_kernel, dim3((unsigned)groups, (unsigned)ceil_div64(k, per)), dim3(TPB), 0, s, x, ld, rows, k, per, left_out, amax);
+  hipLaunchKernelGGL(pack_cols_kernel, dim3((unsigned)ceil_div64(rows, 128), (unsigned)ceil_div64(k, kBlock)), dim3(TPB), 0, s, x, ld, rows, k, left_out,
+                     panels, amax);
+  ENDIA_LAUNCH_CHECK();
+  return ENDIA_HIP_OK;
+}
+
+}  // namespace lce

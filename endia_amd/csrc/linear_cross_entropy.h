@@ -1,0 +1,57 @@
+// Shared parts of the linear cross entropy's kernels for many rows: operands as panels of fp16 pairs and their products.
+//
+// A panel holds 256 rows of an operand [rows, k], k cut into blocks of 32: per block 256 lines of 128 bytes (32 hi, 32 lo of one
+// row; the eight 16-byte pieces swizzled by the row), so that one block of one panel is 32 KiB of consecutive memory and the LDS
+// image that the product kernel reads. k is padded with zeros to a whole block.
+#pragma once
+#include "common.h"
+#include "fp16_pairs.h"
+
+namespace lce {
+
+constexpr int kPanel = 256, kBlock = 32;
+constexpr int64_t kBlockBytes = kPanel * 128;
+
+inline int64_t panel_bytes(int64_t rows, int64_t k) { return ceil_div64(rows, kPanel) * ceil_div64(k, kBlock) * kBlockBytes; }
+
+__device__ __forceinline__ char* line_at(char* panels, int64_t row, int64_t kb, int64_t kblocks) {
+  return panels + ((row / kPanel) * kblocks + kb) * kBlockBytes + (row % kPanel) * 128;
+}
+
+// Source of an operand [rows, k]: element (r, k) at x[r * ld + k], or transposed at x[k * ld + r]. `left_out` (null or one target
+// per index along x's first axis): indices with a negative target are zeros. amax: per row the largest finite magnitude.
+int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax, hipStream_t s);
+
+// z = W x^T piece: A = W rows (classes v0 .. v0 + cols), B = x rows. stats: per 256 classes and row the maximum and the sum of
+// exp(z - maximum); zt: the target's logit, where it lies in the piece.
+struct Logits {
+  const char *w, *x;
+  const float *w_amax, *x_amax, *target;
+  int64_t N, cols, v0, D;
+  float* stats;  // forward: [tiles of classes][N][2]
+  float* zt;
+  const float* lse;    // backward
+  char *p, *pt;        // dz as panels [rows, classes] and [classes, rows]; either may be null
+  int *p_shift, *pt_shift;  // [tiles of classes][N padded], [tiles of rows][cols padded]
+};
+int32_t logits_stats(const Logits& a, hipStream_t s);
+int32_t logits_dz(const Logits& a, hipStream_t s);
+
+// out (+)= c * B A^T: A [rows_a, k] with one scale per row, B [rows_b, k] with one shift per row and 256 of k.
+// element (b, a) at out[b * ld + a], or with by_a at out[a * ld + b]. parts: the walk along k cut into that many; part s goes to
+// out + s * part_stride. c: g[0] / count[0].
+struct Gradient {
+  const char *a, *b;
+  const float* a_amax;
+  const int* b_shift;
+  int64_t b_shift_ld;  // rows of b, padded
+  int64_t rows_a, rows_b, k;
+  float* out;
+  int64_t ld;
+  int by_a, accumulate, parts, vec;  // (vec: set by gradient())
+  int64_t part_stride;
+  const float *g, *count;
+};
+int32_t gradient(const Gradient& a, hipStream_t s);
+
+}  // namespace lce

@@ -7,7 +7,9 @@
 // A row with a negative target is left out: it adds nothing to the loss or to a gradient, whatever x holds there.
 // The forward pass walks the vocabulary once and keeps, per row, the running maximum and the running sum of exp(z - max);
 // the backward pass forms each piece of z again, turns it into dz and multiplies it from both sides.
-#include "common.h"
+// Many rows: products of fp16 pairs (lce_products.hip), the statistics and the cotangents in the products' epilogues.
+// Fewer rows: endia_hip_sgemm on pieces of fp32 logits.
+#include "linear_cross_entropy.h"
 
 using namespace endia;
 
@@ -17,7 +19,15 @@ constexpr int TPB = 256;
 
 struct Scratch {  // a pooled buffer for the time of one call (work on the one stream is ordered, so it can go back at once)
   void* p = nullptr;
+  int64_t used = 0;
   int32_t get(int64_t bytes) { return endia_hip_malloc(bytes, &p); }
+  int64_t want(int64_t bytes) {  // offset of a piece
+    const int64_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    return at;
+  }
+  char* at(int64_t offset) const { return static_cast<char*>(p) + offset; }
+  float* f(int64_t offset) const { return reinterpret_cast<float*>(at(offset)); }
   ~Scratch() {
     if (p) endia_hip_free(p);
   }
@@ -146,6 +156,124 @@ int32_t logits_piece(int64_t N, int64_t D, const float* x, int64_t ldx, int32_t 
                          ENDIA_OP_IDENTITY, nullptr, nullptr, nullptr);
 }
 
+// ---- many rows ------------------------------------------------------------------------------------------------
+constexpr int64_t kManyRows = 512;
+
+// the statistics of a piece's tiles join the running ones of each row
+__global__ __launch_bounds__(TPB) void join_stats_kernel(const float* __restrict__ stats, int64_t tiles, int64_t N, float* __restrict__ m, float* __restrict__ l,
+                                                         int first) {
+  const int64_t n = (int64_t)blockIdx.x * TPB + threadIdx.x;
+  if (n >= N) return;
+  float top = first ? -INFINITY : m[n], sum = first ? 0.f : l[n];
+  for (int64_t t = 0; t < tiles; ++t) {
+    const float2 s = *reinterpret_cast<const float2*>(stats + (t * N + n) * 2);
+    const float now = fmaxf(top, s.x);
+    sum = sum * (top == now ? 1.f : expf(top - now)) + s.y * (s.x == now ? 1.f : expf(s.x - now));
+    top = now;
+  }
+  m[n] = top;
+  l[n] = sum;
+}
+
+__global__ __launch_bounds__(TPB) void add_parts_kernel(const float* __restrict__ part, int64_t n, int parts, float* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x;
+  if (i >= n) return;
+  float sum = part[i];
+  for (int s = 1; s < parts; ++s) sum += part[s * n + i];
+  out[i] = sum;
+}
+
+// classes per piece: panels of the weight's piece of at most 256 MiB, and (backward) at most 2^25 cotangents, 256 MiB as
+// two sets of pairs; a multiple of 256
+int64_t panel_columns(int64_t N, int64_t D, int64_t V, bool backward) {
+  int64_t cols = (64ll << 20) / D;
+  if (backward && cols > (32ll << 20) / N) cols = (32ll << 20) / N;
+  cols = cols / lce::kPanel * lce::kPanel;
+  if (cols < lce::kPanel) cols = lce::kPanel;
+  return cols < V ? cols : V;
+}
+
+int32_t many_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,
+                      float* loss, float* lse, hipStream_t s) {
+  const int64_t piece = panel_columns(N, D, V, false), tiles = ceil_div64(piece, lce::kPanel);
+  Scratch w;
+  const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N), wa = w.want(4 * piece),
+                st = w.want(8 * tiles * N), run = w.want(12 * N);
+  int32_t rc = w.get(w.used);
+  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), s))) return rc;
+  float *m = w.f(run), *l = m + N, *zt = l + N;
+  for (int64_t v0 = 0; v0 < V; v0 += piece) {
+    const int64_t cols = V - v0 < piece ? V - v0 : piece;
+    if ((rc = lce::pack(W + (transW ? v0 * ldw : v0), ldw, !transW, cols, D, nullptr, w.at(wp), w.f(wa), s))) return rc;
+    lce::Logits a = {};
+    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = w.f(wa); a.x_amax = w.f(xa); a.target = target;
+    a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
+    a.stats = w.f(st); a.zt = zt;
+    if ((rc = lce::logits_stats(a, s))) return rc;
+    hipLaunchKernelGGL(join_stats_kernel, dim3((unsigned)ceil_div64(N, TPB)), dim3(TPB), 0, s, w.f(st), ceil_div64(cols, lce::kPanel), N, m, l,
+                       v0 == 0 ? 1 : 0);
+  }
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(TPB), 0, s, N, V, target, m, l, zt, lse, loss);
+  ENDIA_LAUNCH_CHECK();
+  return ENDIA_HIP_OK;
+}
+
+int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,
+                      const float* lse, const float* g, float* dx, float* dW, hipStream_t s) {
+  const int64_t piece = panel_columns(N, D, V, true), rows = ceil_div64(N, lce::kPanel) * lce::kPanel, ptiles = ceil_div64(piece, lce::kPanel);
+  const int64_t dx_tiles = rows / lce::kPanel * ceil_div64(D, lce::kPanel);
+  int parts = (int)ceil_div64(ctx().cu_count, dx_tiles);  // x's gradient has few tiles and a long k: cut k until the chip is full
+  if (parts > ptiles) parts = (int)ptiles;
+  if (parts > 16) parts = 16;
+  Scratch w;
+  const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N), wa = w.want(4 * piece),
+                xt = w.want(dW ? lce::panel_bytes(D, N) : 0), xta = w.want(4 * D), wt = w.want(dx ? lce::panel_bytes(D, piece) : 0), wta = w.want(4 * D),
+                p = w.want(dx ? rows * ptiles * lce::kPanel * 4 : 0), pt = w.want(dW ? rows * ptiles * lce::kPanel * 4 : 0),
+                ps = w.want(4 * ptiles * rows), pts = w.want(4 * rows / lce::kPanel * ptiles * lce::kPanel),
+                dxp = w.want(dx && parts > 1 ? 4 * parts * N * D : 0);
+  int32_t rc = w.get(w.used);
+  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), s))) return rc;
+  if (dW && (rc = lce::pack(x, ldx, true, D, N, target, w.at(xt), w.f(xta), s))) return rc;
+  for (int64_t v0 = 0; v0 < V; v0 += piece) {
+    const int64_t cols = V - v0 < piece ? V - v0 : piece;
+    const float* Wv = W + (transW ? v0 * ldw : v0);
+    if ((rc = lce::pack(Wv, ldw, !transW, cols, D, nullptr, w.at(wp), w.f(wa), s))) return rc;
+    lce::Logits a = {};
+    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = w.f(wa); a.x_amax = w.f(xa); a.target = target;
+    a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
+    a.lse = lse;
+    a.p = dx ? w.at(p) : nullptr;
+    a.pt = dW ? w.at(pt) : nullptr;
+    a.p_shift = reinterpret_cast<int*>(w.at(ps));
+    a.pt_shift = reinterpret_cast<int*>(w.at(pts));
+    if ((rc = lce::logits_dz(a, s))) return rc;
+    lce::Gradient q = {};
+    q.g = g;
+    q.count = lse + N;
+    if (dx) {
+      if ((rc = lce::pack(Wv, ldw, transW, D, cols, nullptr, w.at(wt), w.f(wta), s))) return rc;
+      q.a = w.at(wt); q.b = a.p; q.a_amax = w.f(wta); q.b_shift = a.p_shift; q.b_shift_ld = rows;
+      q.rows_a = D; q.rows_b = N; q.k = cols;
+      q.out = parts > 1 ? w.f(dxp) : dx;
+      q.ld = D; q.by_a = 0; q.accumulate = v0 ? 1 : 0; q.parts = parts; q.part_stride = N * D;
+      if ((rc = lce::gradient(q, s))) return rc;
+    }
+    if (dW) {
+      q.a = w.at(xt); q.b = a.pt; q.a_amax = w.f(xta); q.b_shift = a.pt_shift; q.b_shift_ld = ceil_div64(cols, lce::kPanel) * lce::kPanel;
+      q.rows_a = D; q.rows_b = cols; q.k = N;
+      q.out = transW ? dW + v0 * D : dW + v0;
+      q.ld = transW ? D : V;
+      q.by_a = !transW; q.accumulate = 0; q.parts = 1; q.part_stride = 0;
+      if ((rc = lce::gradient(q, s))) return rc;
+    }
+  }
+  if (dx && parts > 1) {
+    hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)ceil_div64(N * D, TPB)), dim3(TPB), 0, s, w.f(dxp), N * D, parts, dx);
+    ENDIA_LAUNCH_CHECK();
+  }
+  return ENDIA_HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -157,6 +285,7 @@ int32_t endia_hip_linear_cross_entropy_fwd(int64_t N, int64_t D, int64_t V, cons
   ENDIA_CHECK_ARG(loss, "endia_hip_linear_cross_entropy_fwd: null pointer");
   ENDIA_REQUIRE_INIT();
   hipStream_t s = ctx().stream;
+  if (N >= kManyRows) return many_rows_fwd(N, D, V, x, ldx, transW, W, ldw, target, loss, lse, s);
   const int64_t piece = piece_columns(N, V);
   Scratch z, stats;
   if ((rc = z.get(4 * N * piece)) || (rc = stats.get(12 * N))) return rc;
@@ -180,6 +309,7 @@ int32_t endia_hip_linear_cross_entropy_bwd(int64_t N, int64_t D, int64_t V, cons
   ENDIA_CHECK_ARG(dx || dW, "endia_hip_linear_cross_entropy_bwd: nothing to compute");
   ENDIA_REQUIRE_INIT();
   hipStream_t s = ctx().stream;
+  if (N >= kManyRows) return many_rows_bwd(N, D, V, x, ldx, transW, W, ldw, target, lse, g, dx, dW, s);
   const int64_t piece = piece_columns(N, V);
   Scratch z, xk;
   if ((rc = z.get(4 * N * piece))) return rc;
