@@ -25,10 +25,9 @@ __device__ __forceinline__ int bucket_of(const Buckets& t, int rel) {
   } else if (n < 0) {
     n = 0;
   }
-  if (n < t.exact) return base + n;
   int i = t.exact;
-  while (i + 1 < t.side && t.start[i + 1] <= n) ++i;
-  return base + i;
+  for (int j = t.exact + 1; j < t.side; ++j) i += t.start[j] <= n;  // (a uniform index: the starts come through the scalar cache)
+  return base + (n < t.exact ? n : i);
 }
 
 struct Args {
@@ -49,6 +48,7 @@ struct Args {
   float* part;       // partial results of a split walk
   float* part_ml;    // forward: running maximum (base 2) and sum of each partial result
   float* part_table; // per work-group sums of ds by position difference
+  float* part_rows;  // per row and part: sum of ds, sums of p in the two last buckets
   int splits;
   int stages;  // tiles that dq_kernel's LDS holds
   Buckets bk;
@@ -154,6 +154,6 @@ int32_t launch_combine(const Args& a, hipStream_t s);
 int32_t launch_dq(const Args& a, int DP, hipStream_t s);
 int32_t launch_dkv(const Args& a, int DP, hipStream_t s);
 int64_t table_groups(const Args& a);
-int32_t launch_table_grad(const Args& a, float* dtable, hipStream_t s);
+int32_t launch_table_grad(const Args& a, double* diff, float* dtable, hipStream_t s);
 
 }  // namespace attention

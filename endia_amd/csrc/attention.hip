@@ -135,7 +135,7 @@ int32_t endia_hip_attention_fwd(const endia_hip_attention_desc* d, const float* 
   }
   const int DP = padded_dim(a.D);
   const int64_t tiles = ceil_div64(a.K, kTile), images = a.B * a.Hk * tiles * DP * 128;
-  a.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, 2 * cus, tiles, 4);
+  a.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, cus, tiles, 4);
   const int64_t n = a.splits > 1 ? a.B * a.H * a.Q * a.splits : 0;
   const int64_t kr = w.want(images), vc = w.want(images), ks = w.want(4 * a.B * a.Hk * tiles), vs = w.want(4 * a.B * a.Hk * tiles),
                 part = w.want(4 * n * a.D), ml = w.want(8 * n);
@@ -171,15 +171,16 @@ int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* 
   const int64_t kn = a.B * a.Hk * kt, qn = a.B * a.H * qt, image = DP * 128;
   const bool queries = dq || dtable, keys = dk || dv;
   Args aq = a, ak = a;
-  aq.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, 2 * cus, kt, 4);
-  ak.splits = parts(ceil_div64(a.K, 128) * a.Hk * a.B, 2 * cus, a.G * qt, 4);
+  aq.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, cus, kt, 4);
+  ak.splits = parts(ceil_div64(a.K, 128) * a.Hk * a.B, cus, a.G * qt, 4);
   Scratch w;
   const int64_t kr = w.want(kn * image), kc = w.want(kn * image), vr = w.want(kn * image), qr = w.want(qn * image), qc = w.want(qn * image),
                 gr = w.want(qn * image), gc = w.want(qn * image), ksh = w.want(4 * kn), vsh = w.want(4 * kn), qsh = w.want(4 * qn),
                 gsh = w.want(4 * qn), meta = w.want(256 * qn);
   const int64_t part_q = aq.splits > 1 ? 4 * aq.splits * a.B * a.Q * a.H * a.D : 0, part_k = ak.splits > 1 ? 8 * ak.splits * a.B * a.K * a.Hk * a.D : 0;
   const int64_t part = w.want(part_q > part_k ? part_q : part_k);  // (one after the other on the stream)
-  const int64_t table_part = w.want(dtable ? table_groups(aq) * (2 * a.bk.near + 1) * 4 : 0);
+  const int64_t span = 2 * a.bk.near + 1, table_part = w.want(dtable ? table_groups(aq) * span * 4 : 0), diff = w.want(dtable ? 8 * a.H * span : 0),
+                table_rows = w.want(dtable && aq.splits > 1 ? 16 * a.B * a.H * a.Q * aq.splits : 0);
   if ((rc = w.get())) return rc;
   for (Args* x : {&a, &aq, &ak}) {
     x->k_rows = w.at<char>(kr); x->k_cols = w.at<char>(kc); x->v_rows = w.at<char>(vr); x->q_rows = w.at<char>(qr);
@@ -188,10 +189,11 @@ int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* 
     x->meta = w.at<float>(meta);
     x->part = w.at<float>(part);
     x->part_table = dtable ? w.at<float>(table_part) : nullptr;
+    x->part_rows = w.at<float>(table_rows);
   }
   if ((rc = launch_tiles(a, DP, true, st))) return rc;
   if (queries && (rc = launch_dq(aq, DP, st))) return rc;
-  if (dtable && (rc = launch_table_grad(aq, dtable, st))) return rc;
+  if (dtable && (rc = launch_table_grad(aq, w.at<double>(diff), dtable, st))) return rc;
   if (keys && (rc = launch_dkv(ak, DP, st))) return rc;
   return ENDIA_HIP_OK;
 }

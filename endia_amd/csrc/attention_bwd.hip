@@ -16,6 +16,7 @@ namespace {
 
 using namespace pairs;
 constexpr int TPB = 256;
+static_assert(2 * kMaxSide <= TPB, "table_grad_kernel gives every bucket a thread");
 constexpr float kMost = 32768.f;  // a scaled p or ds stays below this
 
 // Brings the running shift F of the lane's accumulator column (2^F times the sums; both halves of the wave agree on it) and the
@@ -107,7 +108,9 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
       for (int j = tid; j < 4 * span; j += TPB) bins[j] = 0.f;
   }
   float* my_bins = bins + wave * span;
-  float far_low = 0.f, far_high = 0.f;
+  // The sum of a row's ds is zero, and a bucket far away holds most of it: what delta is off by (it comes from the rounded o)
+  // would add up there over all keys. So the row's own sum is taken too, and the far buckets give it back by their part of p.
+  float far_low = 0.f, far_high = 0.f, p_low = 0.f, p_high = 0.f, row_sum = 0.f;
 
   const int n = key_count(a, b);
   const int64_t place = i + a.off;
@@ -184,17 +187,32 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
         }
       }
 #pragma unroll
-      for (int v = 0; v < 16; ++v) x[v] = exp2_fast(x[v] - lse) * (dp[v] * cd - delta);
-      // a row without keys has lse = inf here: exp2(-inf) = 0 leaves 0 (dp - delta), which is not 0 if dp is not finite
-      if ((int64_t)(t + 1) * kTile > clear_keys || q0 + 31 >= a.Q) {
+      for (int v = 0; v < 16; ++v) x[v] = exp2_fast(x[v] - lse);
+      // (a row without keys has lse = inf here, which leaves p = 0 but not ds = 0 if dp is not finite)
+      const bool mask = (int64_t)(t + 1) * kTile > clear_keys || q0 + 31 >= a.Q;
+      if (mask) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[v] = in && key0 + 8 * (v >> 2) + (v & 3) < limit ? x[v] : 0.f;
+      }
+      if (sum_table && far) {
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sum += x[v];
+        if (hi <= -near) p_low += sum;
+        else p_high += sum;
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] *= dp[v] * cd - delta;
+      if (mask) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[v] = in && key0 + 8 * (v >> 2) + (v & 3) < limit ? x[v] : 0.f;
       }
       if (sum_table) {
-        if (far) {
-          float sum = 0.f;
+        float sum = 0.f;
 #pragma unroll
-          for (int v = 0; v < 16; ++v) sum += x[v];
+        for (int v = 0; v < 16; ++v) sum += x[v];
+        row_sum += sum;
+        if (far) {
           if (hi <= -near) far_low += sum;
           else far_high += sum;
         } else {
@@ -228,6 +246,19 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
     store_row<DP>(out, dq, c, D, half, a.vec);
   }
   if (sum_table) {
+    // (both halves of the wave hold parts of a row)
+    row_sum += __shfl_xor(row_sum, 32, 64);
+    if (a.splits == 1) {
+      far_low -= row_sum * p_low;
+      far_high -= row_sum * p_high;
+    } else {
+      p_low += __shfl_xor(p_low, 32, 64);
+      p_high += __shfl_xor(p_high, 32, 64);
+      if (in && half == 0) {
+        float* to = a.part_rows + (((b * a.H + h) * a.Q + i) * a.splits + split) * 4;
+        *reinterpret_cast<float4*>(to) = make_float4(row_sum, p_low, p_high, 0.f);
+      }
+    }
     // the wave's far sums join its bins at the ends, then the waves' bins are added in order
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
@@ -409,24 +440,73 @@ __global__ __launch_bounds__(TPB) void reduce_parts_kernel(const float* __restri
   out[i] = sum;
 }
 
-// dtable[bucket, h]: the work-groups' sums by position difference, added in order, in double
-__global__ __launch_bounds__(TPB) void table_grad_kernel(Args a, int64_t groups, float* __restrict__ dtable) {
-  __shared__ double red[TPB];
-  const int span = 2 * a.bk.near + 1, bucket = blockIdx.x;
-  const int64_t h = blockIdx.y, per_head = groups / (a.B * a.H);
+// Sums by position difference of one head over its work-groups, in double and in order: a group of 256 threads takes 64
+// differences and the work-groups in four interleaved runs, which meet in order.
+__global__ __launch_bounds__(TPB) void table_diff_kernel(Args a, int64_t per_head, double* __restrict__ diff) {
+  __shared__ double red[4][64];
+  const int span = 2 * a.bk.near + 1, lane = threadIdx.x & 63, run = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+  const int64_t h = blockIdx.y;
   double sum = 0.0;
-  for (int d = 0; d < span; ++d) {
-    if (bucket_of(a.bk, d - a.bk.near) != bucket) continue;
-    for (int64_t g = threadIdx.x; g < a.B * per_head; g += TPB)
-      sum += (double)a.part_table[(((g / per_head) * a.H + h) * per_head + g % per_head) * span + d];
-  }
-  red[threadIdx.x] = sum;
+  if (d < span)
+    for (int64_t b = 0; b < a.B; ++b) {
+      const float* from = a.part_table + (b * a.H + h) * per_head * span + d;
+#pragma unroll 4
+      for (int64_t g = run; g < per_head; g += 4) sum += (double)from[g * span];
+    }
+  red[run][lane] = sum;
+  __syncthreads();
+  if (run == 0 && d < span) diff[h * span + d] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+
+// dtable[bucket, h] from the sums by difference; what the far buckets give back of their rows' sums where a row was cut in parts.
+__global__ __launch_bounds__(TPB) void table_grad_kernel(Args a, const double* __restrict__ diff, float* __restrict__ dtable) {
+  __shared__ double red[2][TPB];
+  const int span = 2 * a.bk.near + 1, tid = threadIdx.x, buckets = a.bk.both ? 2 * a.bk.side : a.bk.side;
+  const int64_t h = blockIdx.x;
+  double low = 0.0, high = 0.0;
+  if (a.splits > 1)
+    for (int64_t r = tid; r < a.B * a.Q; r += TPB) {
+      const float* from = a.part_rows + ((r / a.Q * a.H + h) * a.Q + r % a.Q) * a.splits * 4;
+      float sum = 0.f, pl = 0.f, ph = 0.f;
+      for (int s = 0; s < a.splits; ++s) {
+        const float4 f = *reinterpret_cast<const float4*>(from + s * 4);
+        sum += f.x;
+        pl += f.y;
+        ph += f.z;
+      }
+      low += (double)(sum * pl);
+      high += (double)(sum * ph);
+    }
+  red[0][tid] = low;
+  red[1][tid] = high;
   __syncthreads();
   for (int s = TPB / 2; s; s >>= 1) {
-    if (threadIdx.x < s) red[threadIdx.x] += red[threadIdx.x + s];
+    if (tid < s) {
+      red[0][tid] += red[0][tid + s];
+      red[1][tid] += red[1][tid + s];
+    }
     __syncthreads();
   }
-  if (threadIdx.x == 0) dtable[bucket * a.H + h] = (float)red[0];
+  // (the differences of a bucket lie side by side; 256 at a time wait in LDS)
+  __shared__ double part[TPB];
+  __shared__ int of[TPB];
+  double sum = 0.0;
+  const int bucket = tid;
+  for (int d0 = 0; d0 < span; d0 += TPB) {
+    __syncthreads();
+    if (d0 + tid < span) {
+      part[tid] = diff[h * span + d0 + tid];
+      of[tid] = bucket_of(a.bk, d0 + tid - a.bk.near);
+    }
+    __syncthreads();
+    if (bucket < buckets)
+      for (int d = 0; d < min(TPB, span - d0); ++d) sum += of[d] == bucket ? part[d] : 0.0;
+  }
+  if (bucket < buckets) {
+    if (bucket == bucket_of(a.bk, -a.bk.near)) sum -= red[0][0];
+    if (bucket == bucket_of(a.bk, a.bk.near)) sum -= red[1][0];
+    dtable[bucket * a.H + h] = (float)sum;
+  }
 }
 
 template <typename Kernel>
@@ -495,8 +575,10 @@ int32_t launch_dkv(const Args& a, int DP, hipStream_t s) {
   return a.dv ? reduce_parts(a.part + n, a.dv, n, 2 * n, a.splits, s) : ENDIA_HIP_OK;
 }
 
-int32_t launch_table_grad(const Args& a, float* dtable, hipStream_t s) {
-  hipLaunchKernelGGL(table_grad_kernel, dim3((unsigned)(a.bk.both ? 2 * a.bk.side : a.bk.side), (unsigned)a.H), dim3(TPB), 0, s, a, table_groups(a), dtable);
+int32_t launch_table_grad(const Args& a, double* diff, float* dtable, hipStream_t s) {
+  const int span = 2 * a.bk.near + 1;
+  hipLaunchKernelGGL(table_diff_kernel, dim3((unsigned)ceil_div64(span, 64), (unsigned)a.H), dim3(TPB), 0, s, a, table_groups(a) / (a.B * a.H), diff);
+  hipLaunchKernelGGL(table_grad_kernel, dim3((unsigned)a.H), dim3(TPB), 0, s, a, diff, dtable);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }

@@ -148,23 +148,42 @@ __global__ __launch_bounds__(TPB) void rows_kernel(Args a) {
   }
 }
 
-// One work-group per row: joins the parts' outputs, each relative to its part's maximum.
-__global__ __launch_bounds__(128) void combine_kernel(Args a) {
-  const int64_t row = blockIdx.x;  // (b H + h) Q + i
-  const int64_t i = row % a.Q, h = row / a.Q % a.H, b = row / a.Q / a.H;
-  const float* ml = a.part_ml + 2 * row * a.splits;
+// One wave per row: joins the parts' outputs, each relative to its part's maximum. The lanes first share the parts' weights out
+// among them.
+__global__ __launch_bounds__(TPB) void combine_kernel(Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (b H + h) Q + i
+  if (row >= a.B * a.H * a.Q) return;
+  const uint32_t bh = (uint32_t)(row / a.Q), i = (uint32_t)(row % a.Q), h = bh % (uint32_t)a.H, b = bh / (uint32_t)a.H;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.splits;
   float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
-  const int d = threadIdx.x;
-  float out = 0.f;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[s].x);
+  top = wave_max(top);
+  float o0 = 0.f, o1 = 0.f;
+  const float* part = a.part + row * a.splits * a.D;
   if (top > -INFINITY)
-    for (int s = 0; s < a.splits; ++s) {
-      const float w = carry(ml[2 * s], top);
-      sum += w * ml[2 * s + 1];
-      if (d < a.D) out += w * a.part[(row * a.splits + s) * a.D + d];
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+      float w = 0.f;
+      if (s0 + lane < a.splits) {
+        const float2 f = ml[s0 + lane];
+        w = carry(f.x, top);
+        sum += w * f.y;
+      }
+      const int n = min(64, a.splits - s0);
+      for (int s = 0; s < n; ++s) {
+        const float ws = __shfl(w, s, 64);
+        const float* from = part + (s0 + s) * a.D;
+        if (lane < a.D) o0 += ws * from[lane];
+        if (lane + 64 < a.D) o1 += ws * from[lane + 64];
+      }
     }
-  if (d < a.D) a.o[((b * a.Q + i) * a.H + h) * a.D + d] = sum != 0.f ? out / sum : 0.f;
-  if (d == 0 && a.lse) a.lse[row] = sum != 0.f ? (top + log2_fast(sum)) * kLn2 : -INFINITY;
+#pragma unroll
+  for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w, 64);
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  float* out = a.o + (((int64_t)b * a.Q + i) * a.H + h) * a.D;
+  if (lane < a.D) out[lane] = o0 * inv;
+  if (lane + 64 < a.D) out[lane + 64] = o1 * inv;
+  if (lane == 0 && a.lse) a.lse[row] = sum != 0.f ? (top + log2_fast(sum)) * kLn2 : -INFINITY;
 }
 
 template <int LPK, int R>
@@ -194,7 +213,7 @@ int32_t launch_rows(const Args& a, int R, hipStream_t s) {
 }
 
 int32_t launch_combine(const Args& a, hipStream_t s) {
-  hipLaunchKernelGGL(combine_kernel, dim3((unsigned)(a.B * a.H * a.Q)), dim3(128), 0, s, a);
+  hipLaunchKernelGGL(combine_kernel, dim3((unsigned)ceil_div64(a.B * a.H * a.Q, 4)), dim3(TPB), 0, s, a);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }

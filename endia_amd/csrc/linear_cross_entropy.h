@@ -54,4 +54,40 @@ struct Gradient {
 };
 int32_t gradient(const Gradient& a, hipStream_t s);
 
+// ---- few rows (lce_direct.hip): the streamed operand [rows, k] in fp32 against N columns held as planes
+inline int64_t plane_bytes(int64_t rows, int64_t k) { return ceil_div64(rows, 32) * ceil_div64(k, 16) * 3072; }
+int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* to, hipStream_t s);
+
+struct Direct {
+  const float* a;
+  int64_t lda, rows, k;
+  const char* planes;
+  int64_t N, v0;
+  int parts;  // the walk along k cut into that many (x's gradient)
+  const float *target, *lse;
+  float *stats, *zt;   // statistics: per 128 classes and row
+  float* dz;           // cotangents [N, rows], row stride dz_ld, or null
+  int64_t dz_ld;
+  char* dz_planes;     // or null
+  float* out;          // x's gradient: [parts][N][rows]
+  int accumulate;
+  const float *g, *count;
+};
+// kcontig: a lies contiguous along k
+int32_t direct_stats(const Direct& p, bool kcontig, hipStream_t s);
+int32_t direct_dz(const Direct& p, bool kcontig, hipStream_t s);
+int32_t direct_dx(const Direct& p, bool kcontig, hipStream_t s);
+
+// out (by_d: [d * ld + v], else [v * ld + d]) = g / count * sum_n x[n, d] dz[n, v]; planes: x's columns along k = n
+struct Outer {
+  const char* planes;
+  const float* dz;
+  int64_t dz_ld, N, D, cols;
+  float* out;
+  int64_t ld;
+  int vec, groups;  // (set by direct_dw)
+  const float *g, *count;
+};
+int32_t direct_dw(const Outer& p, bool by_d, hipStream_t s);
+
 }  // namespace lce
