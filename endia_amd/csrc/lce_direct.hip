@@ -320,31 +320,25 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
         Triple x;
 #pragma unroll
         for (int j = 0; j < 3; ++j) x.p[j] = *reinterpret_cast<const bf16x8*>(stage + ((b * CS + s) * 3 + j) * 1024 + lane * 16);
-        acc[b] = mfma_triples(x, z, acc[b]);
+        acc[b] = BY_D ? mfma_triples(x, z, acc[b]) : mfma_triples(z, x, acc[b]);
       }
     }
     if (turn % chunks == chunks - 1) {
       const int d0 = (g0 + turn / chunks) * DB * 32;
-      if (v < p.cols) {
+      // the axis that lies contiguous in the output is the one along the lanes
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
+      for (int b = 0; b < DB; ++b)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int d = d0 + b * 32 + 8 * q + 4 * half;
-            if (BY_D) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (d + e < p.D) p.out[(int64_t)(d + e) * p.ld + v] = acc[b][4 * q + e] * c;
-            } else if (p.vec) {
-              if (d < p.D)
-                *reinterpret_cast<float4*>(p.out + v * p.ld + d) = make_float4(acc[b][4 * q] * c, acc[b][4 * q + 1] * c, acc[b][4 * q + 2] * c, acc[b][4 * q + 3] * c);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (d + e < p.D) p.out[v * p.ld + d + e] = acc[b][4 * q + e] * c;
-            }
+        for (int i = 0; i < 16; ++i) {
+          const int k = k_of(half, i & 7) + 16 * (i >> 3);
+          if (BY_D) {
+            const int d = d0 + b * 32 + k;
+            if (v < p.cols && d < p.D) p.out[(int64_t)d * p.ld + v] = acc[b][i] * c;
+          } else {
+            const int d = d0 + b * 32 + col;
+            if (d < p.D && v0 + k < p.cols) p.out[(v0 + k) * p.ld + d] = acc[b][i] * c;
           }
-      }
+        }
 #pragma unroll
       for (int b = 0; b < DB; ++b) acc[b] = floatx16{};
     }
@@ -385,7 +379,6 @@ int32_t direct_dx(const Direct& p, bool kcontig, hipStream_t s) { return stream<
 
 int32_t direct_dw(const Outer& q, bool by_d, hipStream_t s) {
   Outer p = q;
-  p.vec = p.D % 4 == 0 && p.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
   const int64_t vg = ceil_div64(p.cols, 128), groups = ceil_div64(p.D, 128);
   int64_t cuts = ceil_div64(4 * endia::ctx().cu_count, vg);  // work-groups along x's columns, when the classes alone do not fill the chip
   if (cuts > groups) cuts = groups;

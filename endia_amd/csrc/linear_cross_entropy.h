@@ -85,7 +85,7 @@ struct Outer {
   int64_t dz_ld, N, D, cols;
   float* out;
   int64_t ld;
-  int vec, groups;  // (set by direct_dw)
+  int groups;  // of 128 of x's columns per work-group (set by direct_dw)
   const float *g, *count;
 };
 int32_t direct_dw(const Outer& p, bool by_d, hipStream_t s);

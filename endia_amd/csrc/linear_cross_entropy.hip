@@ -107,13 +107,20 @@ __global__ __launch_bounds__(TPB) void join_stats_kernel(const float* __restrict
   }
 }
 
-// out[r * ld + c] = the sum of the parts' [rows, cols], in order
+// out[r * ld + c] = the sum of the parts' [rows, cols]: a work-group takes 64 elements and the parts in four interleaved runs, which
+// meet in order
 __global__ __launch_bounds__(TPB) void add_parts_kernel(const float* __restrict__ part, int64_t rows, int64_t cols, int parts, float* __restrict__ out, int64_t ld) {
-  const int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x, n = rows * cols;
-  if (i >= n) return;
-  float sum = part[i];
-  for (int s = 1; s < parts; ++s) sum += part[s * n + i];
-  out[i / cols * ld + i % cols] = sum;
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane, n = rows * cols;
+  float sum = 0.f;
+  if (i < n) {
+#pragma unroll 8
+    for (int s = run; s < parts; s += 4) sum += part[s * n + i];
+  }
+  red[run][lane] = sum;
+  __syncthreads();
+  if (run == 0 && i < n) out[i / cols * ld + i % cols] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
 int32_t join_stats(const float* stats, int64_t tiles, int64_t N, float* m, float* l, bool first, hipStream_t s) {
@@ -123,7 +130,7 @@ int32_t join_stats(const float* stats, int64_t tiles, int64_t N, float* m, float
 }
 
 int32_t add_parts(const float* part, int64_t rows, int64_t cols, int parts, float* out, int64_t ld, hipStream_t s) {
-  hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)ceil_div64(rows * cols, TPB)), dim3(TPB), 0, s, part, rows, cols, parts, out, ld);
+  hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)ceil_div64(rows * cols, 64)), dim3(TPB), 0, s, part, rows, cols, parts, out, ld);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }
