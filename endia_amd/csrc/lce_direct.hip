@@ -1,16 +1,21 @@
 // The linear cross entropy for few rows (up to a few hundred): the weight is what there is to read, so it is read as it lies, in
 // fp32 and in either storage order, straight into matrix operands; no copy of it in another form is made.
 //
-// An fp32 number is held as three bf16 (hi, mid, lo: 8 + 8 + 8 bits, with fp32's exponent, so nothing has to be scaled and no pass
-// over the weight has to find a maximum first). A product is six bf16 products,
+// Up to 64 rows an fp32 number is held as three bf16 (hi, mid, lo: 8 + 8 + 8 bits, with fp32's exponent, so nothing has to be
+// scaled and no pass over the weight has to find a maximum first). A product is six bf16 products,
 //   x y = hi hi + hi mid + mid hi + hi lo + mid mid + lo hi   (the rest is below 2^-24 of it),
-// accumulated in fp32. The small operand (x, or the cotangents) is turned into such triples once, in operand order ("planes").
+// accumulated in fp32: HBM is the bound, the matrix pipe has the time. Beyond 64 rows it has not, and the operands are pairs of
+// fp16 (fp16_pairs.h: three products), scaled by the largest magnitude of each class's weights, which the forward pass finds in a
+// pass of its own and leaves for the backward pass. The cotangents as an operand of x's gradient stay bf16 triples: a row that is
+// nearly right has cotangents far below 1, and no one scale fits all of its classes.
+// The small operand (x, or the cotangents) is brought into operand order once ("planes").
 //
-// A work-group of 4 waves takes 128 rows of the streamed operand (32 per wave) against up to 128 columns; the waves share the
-// columns' planes through LDS, and the next chunk of both travels while this one is multiplied.
-// Bound: HBM up to about 96 columns (per 2 KiB of weight and wave 6 x 32 cycles of the matrix pipe per 32 columns and about 200 of
-// the vector ALU, against some 900 cycles that its share of the memory takes), the matrix pipe beyond.
+// up to 32 rows of x (stream_few_kernel): a work-group takes 32 rows of the streamed operand, its four waves share k out among
+// them without a barrier and add up in LDS. More (stream_kernel): 128 rows, 32 per wave, against up to 128 columns, whose planes
+// the waves share through LDS; the next chunk of both operands travels while this one is multiplied.
 #include "linear_cross_entropy.h"
+
+#include <type_traits>
 
 namespace lce {
 
@@ -25,14 +30,22 @@ constexpr int TPB = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 // Cotangents, at most 1, are held times 2^40, so that the lower parts of hardly likely classes stay in bf16's normal range.
 constexpr int kUp = 40;
-constexpr int kStepBytes = 3 * 1024;  // planes of 32 columns x 16 of k
+// planes of 32 columns x 16 of k: 1 KiB for each part
+template <typename Op>
+constexpr int step_bytes() { return Op::PARTS * 1024; }
 
 struct Triple {
+  static constexpr int PARTS = 3;
+  typedef bf16x8 Vec;
   bf16x8 p[3];
 };
+struct Pair {
+  static constexpr int PARTS = 2;
+  typedef pairs::half8 Vec;
+  pairs::half8 p[2];
+};
 
-__device__ __forceinline__ Triple triple(const float (&x)[8]) {
-  Triple t;
+__device__ __forceinline__ void split(const float (&x)[8], int, Triple& t) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     float2v r = {x[i], x[i + 1]};
@@ -45,12 +58,18 @@ __device__ __forceinline__ Triple triple(const float (&x)[8]) {
       r[1] -= (float)h[1];
     }
   }
-  return t;
+}
+__device__ __forceinline__ void split(const float (&x)[8], int shift, Pair& t) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = pairs::scaled(x[e], shift);
+  pairs::split8(y, t.p[0], t.p[1]);
 }
 
 __device__ __forceinline__ floatx16 mfma(bf16x8 a, bf16x8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-__device__ __forceinline__ floatx16 mfma_triples(const Triple& a, const Triple& b, floatx16 c) {
+__device__ __forceinline__ floatx16 multiply(const Pair& a, const Pair& b, floatx16 c) { return pairs::mfma_pairs(a.p[0], a.p[1], b.p[0], b.p[1], c); }
+__device__ __forceinline__ floatx16 multiply(const Triple& a, const Triple& b, floatx16 c) {
   c = mfma(a.p[2], b.p[0], c);
   c = mfma(a.p[1], b.p[1], c);
   c = mfma(a.p[0], b.p[2], c);
@@ -88,10 +107,10 @@ __device__ __forceinline__ void load_step(const float* __restrict__ x, int64_t l
   }
 }
 
-// Planes of an operand [rows, k]: per 32 rows and step of 16: hi, mid, lo, each 64 lanes x 16 bytes. One wave per step.
-template <bool KCONTIG>
+// Planes of an operand [rows, k]: per 32 rows and step of 16 the parts, each 64 lanes x 16 bytes. One wave per step.
+template <bool KCONTIG, typename Op>
 __global__ __launch_bounds__(TPB) void planes_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, const float* __restrict__ left_out,
-                                                     char* __restrict__ planes) {
+                                                     const float* __restrict__ amax, char* __restrict__ planes) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int64_t steps = (k + 15) / 16, step = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), block = blockIdx.y, r = block * 32 + (lane & 31);
   if (step >= steps) return;
@@ -103,18 +122,148 @@ __global__ __launch_bounds__(TPB) void planes_kernel(const float* __restrict__ x
     const bool skip = r >= rows || (left_out && i < (KCONTIG ? rows : k) && left_out[i] < 0.f);
     v[e] = skip ? 0.f : v[e];
   }
-  const Triple t = triple(v);
-  char* to = planes + (block * steps + step) * kStepBytes + lane * 16;
+  Op t;
+  split(v, amax ? pairs::shift_of(amax[min(r, rows - 1)]) : 0, t);
+  char* to = planes + (block * steps + step) * step_bytes<Op>() + lane * 16;
 #pragma unroll
-  for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(to + j * 1024) = t.p[j];
+  for (int j = 0; j < Op::PARTS; ++j) *reinterpret_cast<typename Op::Vec*>(to + j * 1024) = t.p[j];
 }
 
 enum { STATS, DZ, DX };
 
-template <int NB, bool KCONTIG, bool VEC, int MODE>
+template <typename Op>
+__device__ __forceinline__ Op read_planes(const char* from, int lane) {
+  Op x;
+#pragma unroll
+  for (int j = 0; j < Op::PARTS; ++j) x.p[j] = *reinterpret_cast<const typename Op::Vec*>(from + j * 1024 + lane * 16);
+  return x;
+}
+
+// What becomes of 32 rows of the streamed operand (from r0, `left` of them there) against 32 rows n of x: z of the lane's n in acc.
+// Maximum and sum of exp over the rows:
+__device__ __forceinline__ void stats_block(const Direct& p, floatx16& acc, int64_t r0, int left, int n, int half, float& m, float& sum) {
+  m = -INFINITY;
+  sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int i = k_of(half, v & 7) + 16 * (v >> 3);
+    acc[v] = i < left ? acc[v] : -INFINITY;
+    m = fmaxf(m, acc[v]);
+  }
+  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  const float top = m * kLog2e;
+  const float t = n < p.N ? p.target[n] : -1.f, local = t - (float)(p.v0 + r0);
+  const int hot = local >= 0.f && local < 32.f ? (int)local : -1;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const float z = acc[v];
+    if (hot == k_of(half, v & 7) + 16 * (v >> 3) && hot < left) p.zt[n] = z;
+    sum += z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -top));
+  }
+  sum += __shfl_xor(sum, 32, 64);
+}
+
+// Cotangents: fp32 [N, rows] for the weight's gradient, and as planes (columns: rows of x, k: classes) for x's.
+__device__ __forceinline__ void dz_block(const Direct& p, const floatx16& acc, int64_t r0, int left, int n, int block, int lane, int half) {
+  const int64_t zsteps = (p.rows + 15) / 16;
+  const float t = n < p.N ? p.target[n] : -1.f, e = p.lse[min((int64_t)n, p.N - 1)] * kLog2e - (float)kUp, local = t - (float)(p.v0 + r0);
+  const int hot = local >= 0.f && local < 32.f ? (int)local : -1;
+  float d[2][8];
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int i = k_of(half, v & 7) + 16 * (v >> 3);
+    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], kLog2e, -e)) - (i == hot ? (float)(1ll << kUp) : 0.f);
+    d[v >> 3][v & 7] = i < left && !(t < 0.f) ? y : 0.f;
+  }
+  if (p.dz && n < p.N) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int i = k_of(half, v & 7) + 16 * (v >> 3);
+      if (i < left) p.dz[(int64_t)n * p.dz_ld + r0 + i] = d[v >> 3][v & 7];
+    }
+  }
+  if (p.dz_planes && block * 32 < p.N)
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (16 * s < left) {
+        Triple y;
+        split(d[s], 0, y);
+        char* to = p.dz_planes + ((int64_t)block * zsteps + r0 / 16 + s) * step_bytes<Triple>() + lane * 16;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(to + j * 1024) = y.p[j];
+      }
+}
+
+__device__ __forceinline__ void dx_block(const Direct& p, const floatx16& acc, int64_t r0, int left, int n, int half, int part) {
+  if (n >= p.N) return;
+  const float c = p.count[0] > 0.f ? __builtin_ldexpf(p.g[0] / p.count[0], -kUp) : 0.f;
+  float* out = p.out + ((int64_t)part * p.N + n) * p.rows + r0;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int i = k_of(half, v & 7) + 16 * (v >> 3);
+    if (i < left) out[i] = p.accumulate ? out[i] + acc[v] * c : acc[v] * c;
+  }
+}
+
+// Up to 32 rows of x. Waves take chunks of 4 steps in turn; nothing is shared until the end.
+template <bool KCONTIG, bool VEC, int MODE>
+__global__ __launch_bounds__(TPB, 2) void stream_few_kernel(Direct p) {
+  constexpr int CS = 4;
+  __shared__ float red[4][16][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * 32;
+  const int part = blockIdx.z;
+  const int steps = (int)((p.k + 15) / 16), chunks = (steps + CS - 1) / CS, per = (chunks + p.parts - 1) / p.parts;
+  const int c0 = min(part * per, chunks), c1 = min(c0 + per, chunks);
+  float next[CS][8], now[CS][8];
+  Triple xn[CS], x[CS];
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      load_step<KCONTIG, VEC>(p.a, p.lda, r0 + col, p.rows, (int64_t)(c * CS + s) * 16, p.k, half, next[s]);
+      xn[s] = read_planes<Triple>(p.planes + (int64_t)min(c * CS + s, steps - 1) * step_bytes<Triple>(), lane);
+    }
+  };
+  floatx16 acc = {};
+  int c = c0 + wave;
+  if (c < c1) fetch(c);
+  for (; c < c1; c += 4) {
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      x[s] = xn[s];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) now[s][e] = next[s][e];
+    }
+    if (c + 4 < c1) fetch(c + 4);
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      Triple a;
+      split(now[s], 0, a);
+      acc = multiply(a, x[s], acc);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < 16; ++v) red[wave][v][lane] = acc[v];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) acc[v] = (red[0][v][lane] + red[1][v][lane]) + (red[2][v][lane] + red[3][v][lane]);
+  const int left = (int)min(p.rows - r0, (int64_t)32);
+  if (MODE == STATS) {
+    float m, sum;
+    stats_block(p, acc, r0, left, col, half, m, sum);
+    if (half == 0 && col < p.N) *reinterpret_cast<float2*>(p.stats + ((int64_t)blockIdx.x * p.N + col) * 2) = make_float2(m, sum);
+  } else if (MODE == DZ) {
+    dz_block(p, acc, r0, left, col, 0, lane, half);
+  } else {
+    dx_block(p, acc, r0, left, col, half, part);
+  }
+}
+
+template <int NB, typename Op, bool KCONTIG, bool VEC, int MODE>
 __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
-  constexpr int CS = NB == 4 ? 2 : 4;                // steps per chunk
-  constexpr int STAGE = CS * NB * kStepBytes;
+  constexpr int CS = NB > 2 ? 2 : 4;  // steps per chunk
+  constexpr int STAGE = CS * NB * step_bytes<Op>(), P = Op::PARTS;
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * 128 + wave * 32;
@@ -122,16 +271,17 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   const int steps = (int)((p.k + 15) / 16), chunks = (steps + CS - 1) / CS, per = (chunks + p.parts - 1) / p.parts;
   const int c0 = min(part * per, chunks), c1 = min(c0 + per, chunks);
   const int blocks = (int)((p.N + 31) / 32), first_block = n0 / 32;
+  const int shift = P == 2 ? pairs::shift_of(p.a_amax[min(r0 + col, p.rows - 1)]) : 0;
 
   // planes of chunk c: NB blocks of columns, CS steps each (clamped: a step or block behind the end is read again and not used)
   auto request = [&](int c, char* to) {
-    constexpr int LINES = CS * NB * 3;  // of 1 KiB
+    constexpr int LINES = CS * NB * P;  // of 1 KiB
 #pragma unroll
     for (int i = 0; i < (LINES + 3) / 4; ++i) {
       const int line = i * 4 + wave;
       if (LINES % 4 == 0 || line < LINES) {
-        const int b = line / (CS * 3), s = line / 3 % CS, j = line % 3;
-        const int64_t from = ((int64_t)min(first_block + b, blocks - 1) * steps + min(c * CS + s, steps - 1)) * kStepBytes + j * 1024;
+        const int b = line / (CS * P), s = line / P % CS, j = line % P;
+        const int64_t from = ((int64_t)min(first_block + b, blocks - 1) * steps + min(c * CS + s, steps - 1)) * step_bytes<Op>() + j * 1024;
         pairs::load_to_lds(p.planes + from + lane * 16, to + line * 1024);
       }
     }
@@ -162,16 +312,24 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
     }
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
-      const Triple a = triple(now[s]);
+      Op a;
+      split(now[s], shift, a);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        Triple x;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) x.p[j] = *reinterpret_cast<const bf16x8*>(stage + ((b * CS + s) * 3 + j) * 1024 + lane * 16);
-        acc[b] = mfma_triples(a, x, acc[b]);
-      }
+      for (int b = 0; b < NB; ++b) acc[b] = multiply(a, read_planes<Op>(stage + (b * CS + s) * step_bytes<Op>(), lane), acc[b]);
     }
     pairs::wait_loads();
+    __syncthreads();
+  }
+  if (P == 2) {  // the scales come off: of the columns per lane, of the rows per register
+    float* down = reinterpret_cast<float*>(smem) + wave * 32;
+    if (half == 0) down[col] = __builtin_ldexpf(1.f, -shift);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float cx = __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min((int64_t)n0 + b * 32 + col, p.N - 1)]));
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[b][v] = acc[b][v] * cx * down[k_of(half, v & 7) + 16 * (v >> 3)];
+    }
     __syncthreads();
   }
 
@@ -180,29 +338,9 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
     float* red = reinterpret_cast<float*>(smem);  // [4 waves][NB * 32][2]
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int n = n0 + b * 32 + col;
-      float m = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int i = k_of(half, v & 7) + 16 * (v >> 3);
-        acc[b][v] = i < left ? acc[b][v] : -INFINITY;
-        m = fmaxf(m, acc[b][v]);
-      }
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float top = m * kLog2e;
-      const float t = n < p.N ? p.target[n] : -1.f, local = t - (float)(p.v0 + r0);
-      const int hot = local >= 0.f && local < 32.f ? (int)local : -1;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const float z = acc[b][v];
-        if (hot == k_of(half, v & 7) + 16 * (v >> 3) && hot < left) p.zt[n] = z;
-        sum += z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -top));
-      }
-      sum += __shfl_xor(sum, 32, 64);
-      if (half == 0) {
-        red[(wave * NB * 32 + b * 32 + col) * 2] = m;
-        red[(wave * NB * 32 + b * 32 + col) * 2 + 1] = sum;
-      }
+      float m, sum;
+      stats_block(p, acc[b], r0, left, n0 + b * 32 + col, half, m, sum);
+      if (half == 0) *reinterpret_cast<float2*>(red + (wave * NB * 32 + b * 32 + col) * 2) = make_float2(m, sum);
     }
     __syncthreads();
     if (tid < NB * 32 && n0 + tid < p.N) {
@@ -212,64 +350,22 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
         const float mw = red[(w * NB * 32 + tid) * 2], lw = red[(w * NB * 32 + tid) * 2 + 1];
         sum += lw == 0.f ? 0.f : lw * __builtin_amdgcn_exp2f((mw - m) * kLog2e);
       }
-      float* to = p.stats + ((int64_t)blockIdx.x * p.N + n0 + tid) * 2;
-      to[0] = m;
-      to[1] = sum;
-    }
-  } else if (MODE == DZ) {
-    // cotangents: fp32 [N, rows] for the weight's gradient, and as planes (columns: rows of x, k: classes) for x's
-    const int64_t zsteps = (p.rows + 15) / 16;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int n = n0 + b * 32 + col;
-      const float t = n < p.N ? p.target[n] : -1.f, e = p.lse[min((int64_t)n, p.N - 1)] * kLog2e - (float)kUp, local = t - (float)(p.v0 + r0);
-      const int hot = local >= 0.f && local < 32.f ? (int)local : -1;
-      float d[2][8];
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int i = k_of(half, v & 7) + 16 * (v >> 3);
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][v], kLog2e, -e)) - (i == hot ? (float)(1ll << kUp) : 0.f);
-        d[v >> 3][v & 7] = i < left && !(t < 0.f) ? y : 0.f;
-      }
-      if (p.dz && n < p.N) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int i = k_of(half, v & 7) + 16 * (v >> 3);
-          if (i < left) p.dz[(int64_t)n * p.dz_ld + r0 + i] = d[v >> 3][v & 7];
-        }
-      }
-      if (p.dz_planes && first_block + b < blocks)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-          if (16 * s < left) {
-            const Triple y = triple(d[s]);
-            char* to = p.dz_planes + ((int64_t)(first_block + b) * zsteps + r0 / 16 + s) * kStepBytes + lane * 16;
-#pragma unroll
-            for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(to + j * 1024) = y.p[j];
-          }
+      *reinterpret_cast<float2*>(p.stats + ((int64_t)blockIdx.x * p.N + n0 + tid) * 2) = make_float2(m, sum);
     }
   } else {
-    const float c = p.count[0] > 0.f ? __builtin_ldexpf(p.g[0] / p.count[0], -kUp) : 0.f;
-    float* out = p.out + part * p.N * p.rows;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int n = n0 + b * 32 + col;
-      if (n >= p.N) continue;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int i = k_of(half, v & 7) + 16 * (v >> 3);
-        float* to = out + n * p.rows + r0 + i;
-        if (i < left) *to = p.accumulate ? *to + acc[b][v] * c : acc[b][v] * c;
-      }
+      if (MODE == DZ) dz_block(p, acc[b], r0, left, n0 + b * 32 + col, first_block + b, lane, half);
+      else dx_block(p, acc[b], r0, left, n0 + b * 32 + col, half, part);
     }
   }
 }
 
 // dW[d, v] = c sum_n x[n, d] dz[n, v]: a wave takes 32 classes against 4 x 32 of x's columns at a time, whose planes the four waves
 // share through LDS. Bound: HBM (the gradient is written once) up to about 128 rows.
-template <bool BY_D>
+template <bool BY_D, typename Op>
 __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
-  constexpr int DB = 4, CS = 2, STAGE = DB * CS * kStepBytes;
+  constexpr int DB = 4, CS = 2, P = Op::PARTS, STAGE = DB * CS * step_bytes<Op>();
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int64_t v0 = (int64_t)blockIdx.x * 128 + wave * 32, v = v0 + col;
@@ -280,12 +376,20 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
   auto request = [&](int turn, char* to) {
     const int g = g0 + turn / chunks, ch = turn % chunks;
 #pragma unroll
-    for (int i = 0; i < DB * CS * 3 / 4; ++i) {
-      const int line = i * 4 + wave, b = line / (CS * 3), s = line / 3 % CS, j = line % 3;
-      const int64_t from = ((int64_t)min(g * DB + b, blocks - 1) * steps + min(ch * CS + s, steps - 1)) * kStepBytes + j * 1024;
+    for (int i = 0; i < DB * CS * P / 4; ++i) {
+      const int line = i * 4 + wave, b = line / (CS * P), s = line / P % CS, j = line % P;
+      const int64_t from = ((int64_t)min(g * DB + b, blocks - 1) * steps + min(ch * CS + s, steps - 1)) * step_bytes<Op>() + j * 1024;
       pairs::load_to_lds(p.planes + from + lane * 16, to + line * 1024);
     }
   };
+  int shift = 0;
+  if (P == 2) {  // the scale of the class's cotangents over the rows
+    float amax = 0.f;
+    const float* z = p.dz + min(v, p.cols - 1);
+#pragma unroll 8
+    for (int64_t n = half; n < p.N; n += 2) amax = fmaxf(amax, pairs::finite_abs(z[n * p.dz_ld]));
+    shift = pairs::shift_of(fmaxf(amax, __shfl_xor(amax, 32, 64)));
+  }
   float next[CS][8], now[CS][8];
   auto fetch = [&](int turn) {
     const int ch = turn % chunks;
@@ -314,18 +418,28 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
       if ((turn % chunks) * CS + s >= steps) break;
-      const Triple z = triple(now[s]);
+      Op z;
+      split(now[s], shift, z);
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
-        Triple x;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) x.p[j] = *reinterpret_cast<const bf16x8*>(stage + ((b * CS + s) * 3 + j) * 1024 + lane * 16);
-        acc[b] = BY_D ? mfma_triples(x, z, acc[b]) : mfma_triples(z, x, acc[b]);
+        const Op x = read_planes<Op>(stage + (b * CS + s) * step_bytes<Op>(), lane);
+        acc[b] = BY_D ? multiply(x, z, acc[b]) : multiply(z, x, acc[b]);
       }
     }
     if (turn % chunks == chunks - 1) {
       const int d0 = (g0 + turn / chunks) * DB * 32;
       // the axis that lies contiguous in the output is the one along the lanes
+      if (P == 2) {
+        const float down_v = __builtin_ldexpf(1.f, -shift);  // of the lane's class: with classes along the registers, lane k has theirs
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int k = k_of(half, i & 7) + 16 * (i >> 3), d = d0 + b * 32 + (BY_D ? k : col);
+            const float down_x = __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min(d, (int)p.D - 1)]));
+            acc[b][i] *= down_x * (BY_D ? down_v : __shfl(down_v, k, 64));
+          }
+      }
 #pragma unroll
       for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -347,32 +461,48 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
   }
 }
 
-template <int NB, int MODE>
+template <int NB, typename Op, int MODE>
 int32_t stream(const Direct& p, bool kcontig, bool vec, hipStream_t s) {
   const dim3 grid((unsigned)ceil_div64(p.rows, 128), (unsigned)ceil_div64(p.N, NB * 32), (unsigned)p.parts);
-  if (!kcontig) hipLaunchKernelGGL((stream_kernel<NB, false, false, MODE>), grid, dim3(TPB), 0, s, p);
-  else if (vec) hipLaunchKernelGGL((stream_kernel<NB, true, true, MODE>), grid, dim3(TPB), 0, s, p);
-  else hipLaunchKernelGGL((stream_kernel<NB, true, false, MODE>), grid, dim3(TPB), 0, s, p);
+  if (!kcontig) hipLaunchKernelGGL((stream_kernel<NB, Op, false, false, MODE>), grid, dim3(TPB), 0, s, p);
+  else if (vec) hipLaunchKernelGGL((stream_kernel<NB, Op, true, true, MODE>), grid, dim3(TPB), 0, s, p);
+  else hipLaunchKernelGGL((stream_kernel<NB, Op, true, false, MODE>), grid, dim3(TPB), 0, s, p);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }
 
+// Op: operands of statistics and cotangents beyond kTripleRows rows of x are pairs, all others triples
 template <int MODE>
 int32_t stream(const Direct& p, bool kcontig, hipStream_t s) {
+  using Op = typename std::conditional<MODE == DX, Triple, Pair>::type;
   const bool vec = kcontig && p.lda % 4 == 0 && p.k % 4 == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
-  return p.N <= 32 ? stream<1, MODE>(p, kcontig, vec, s) : p.N <= 64 ? stream<2, MODE>(p, kcontig, vec, s) : stream<4, MODE>(p, kcontig, vec, s);
+  if (p.N <= 32) {
+    const dim3 grid((unsigned)ceil_div64(p.rows, 32), 1, (unsigned)p.parts);
+    if (!kcontig) hipLaunchKernelGGL((stream_few_kernel<false, false, MODE>), grid, dim3(TPB), 0, s, p);
+    else if (vec) hipLaunchKernelGGL((stream_few_kernel<true, true, MODE>), grid, dim3(TPB), 0, s, p);
+    else hipLaunchKernelGGL((stream_few_kernel<true, false, MODE>), grid, dim3(TPB), 0, s, p);
+    ENDIA_LAUNCH_CHECK();
+    return ENDIA_HIP_OK;
+  }
+  if (p.N <= kTripleRows) return stream<2, Triple, MODE>(p, kcontig, vec, s);
+  // 96 or 128 columns at a time, whichever leaves fewer of them empty
+  const int64_t blocks = ceil_div64(p.N, 32);
+  return ceil_div64(blocks, 3) * 3 < ceil_div64(blocks, 4) * 4 ? stream<3, Op, MODE>(p, kcontig, vec, s) : stream<4, Op, MODE>(p, kcontig, vec, s);
 }
 
 }  // namespace
 
-int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* to, hipStream_t s) {
+int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, const float* amax, char* to, hipStream_t s) {
   const dim3 grid((unsigned)ceil_div64(ceil_div64(k, 16), 4), (unsigned)ceil_div64(rows, 32));
-  if (transposed) hipLaunchKernelGGL(planes_kernel<false>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, to);
-  else hipLaunchKernelGGL(planes_kernel<true>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, to);
+  if (transposed && amax) hipLaunchKernelGGL((planes_kernel<false, Pair>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);
+  else if (transposed) hipLaunchKernelGGL((planes_kernel<false, Triple>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);
+  else if (amax) hipLaunchKernelGGL((planes_kernel<true, Pair>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);
+  else hipLaunchKernelGGL((planes_kernel<true, Triple>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }
 
+int64_t direct_rows(int64_t N) { return N <= 32 ? 32 : 128; }
 int32_t direct_stats(const Direct& p, bool kcontig, hipStream_t s) { return stream<STATS>(p, kcontig, s); }
 int32_t direct_dz(const Direct& p, bool kcontig, hipStream_t s) { return stream<DZ>(p, kcontig, s); }
 int32_t direct_dx(const Direct& p, bool kcontig, hipStream_t s) { return stream<DX>(p, kcontig, s); }
@@ -384,8 +514,13 @@ int32_t direct_dw(const Outer& q, bool by_d, hipStream_t s) {
   if (cuts > groups) cuts = groups;
   p.groups = (int)ceil_div64(groups, cuts);
   const dim3 grid((unsigned)vg, (unsigned)ceil_div64(groups, p.groups));
-  if (by_d) hipLaunchKernelGGL(outer_kernel<true>, grid, dim3(TPB), 0, s, p);
-  else hipLaunchKernelGGL(outer_kernel<false>, grid, dim3(TPB), 0, s, p);
+  if (p.x_amax) {
+    if (by_d) hipLaunchKernelGGL((outer_kernel<true, Pair>), grid, dim3(TPB), 0, s, p);
+    else hipLaunchKernelGGL((outer_kernel<false, Pair>), grid, dim3(TPB), 0, s, p);
+  } else {
+    if (by_d) hipLaunchKernelGGL((outer_kernel<true, Triple>), grid, dim3(TPB), 0, s, p);
+    else hipLaunchKernelGGL((outer_kernel<false, Triple>), grid, dim3(TPB), 0, s, p);
+  }
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }

@@ -23,7 +23,7 @@ __device__ __forceinline__ void store_chunk(char* line, int row, int chunk, cons
 // Source rows contiguous along k: one wave per row, the row twice (the second time from cache).
 template <bool VEC>
 __global__ __launch_bounds__(TPB) void pack_rows_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, const float* __restrict__ left_out,
-                                                        char* __restrict__ panels, float* __restrict__ amax_out) {
+                                                        char* __restrict__ panels, float* __restrict__ amax_out, int known) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(TPB) void pack_rows_kernel(const float* __restrict_
       for (int e = 0; e < 8; ++e) v[e] = k0 + e < k ? r[k0 + e] : 0.f;
     }
   };
-  if (!skip)
+  if (!skip && !known)
     for (int64_t k0 = lane * 8; k0 < k; k0 += 512) {
       float v[8];
       load8(k0, v);
@@ -52,7 +52,9 @@ __global__ __launch_bounds__(TPB) void pack_rows_kernel(const float* __restrict_
     }
 #pragma unroll
   for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-  if (lane == 0) amax_out[row] = amax;
+  if (known) amax = amax_out[row];
+  else if (lane == 0) amax_out[row] = amax;
+  if (!panels) return;
   const int shift = shift_of(amax);
   const int64_t kblocks = (k + kBlock - 1) / kBlock;
   for (int64_t k0 = lane * 8; k0 < kblocks * kBlock; k0 += 512) {
@@ -111,15 +113,8 @@ __global__ __launch_bounds__(TPB) void pack_cols_kernel(const float* __restrict_
 
 }  // namespace
 
-int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax, hipStream_t s) {
-  if (!transposed) {
-    const bool vec = k % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    const dim3 grid((unsigned)ceil_div64(rows, 4));
-    if (vec) hipLaunchKernelGGL(pack_rows_kernel<true>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax);
-    else hipLaunchKernelGGL(pack_rows_kernel<false>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax);
-    ENDIA_LAUNCH_CHECK();
-    return ENDIA_HIP_OK;
-  }
+int32_t row_amax(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, float* amax, hipStream_t s) {
+  if (!transposed) return pack(x, ld, false, rows, k, left_out, nullptr, amax, false, s);
   hipLaunchKernelGGL(zero_kernel, dim3((unsigned)ceil_div64(rows, TPB)), dim3(TPB), 0, s, amax, rows);
   const int64_t groups = ceil_div64(rows, TPB);
   int64_t cuts = ceil_div64(4096, groups);
@@ -127,6 +122,22 @@ int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t 
   if (cuts > 65535) cuts = 65535;
   const int64_t per = ceil_div64(k, cuts);
   hipLaunchKernelGGL(col_amax_kernel, dim3((unsigned)groups, (unsigned)ceil_div64(k, per)), dim3(TPB), 0, s, x, ld, rows, k, per, left_out, amax);
+  ENDIA_LAUNCH_CHECK();
+  return ENDIA_HIP_OK;
+}
+
+int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax, bool known,
+             hipStream_t s) {
+  if (!transposed) {
+    const bool vec = k % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    const dim3 grid((unsigned)ceil_div64(rows, 4));
+    if (vec) hipLaunchKernelGGL(pack_rows_kernel<true>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax, known ? 1 : 0);
+    else hipLaunchKernelGGL(pack_rows_kernel<false>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax, known ? 1 : 0);
+    ENDIA_LAUNCH_CHECK();
+    return ENDIA_HIP_OK;
+  }
+  int32_t rc = known ? ENDIA_HIP_OK : row_amax(x, ld, true, rows, k, left_out, amax, s);
+  if (rc) return rc;
   hipLaunchKernelGGL(pack_cols_kernel, dim3((unsigned)ceil_div64(rows, 128), (unsigned)ceil_div64(k, kBlock)), dim3(TPB), 0, s, x, ld, rows, k, left_out,
                      panels, amax);
   ENDIA_LAUNCH_CHECK();

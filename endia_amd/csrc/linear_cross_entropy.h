@@ -20,7 +20,8 @@ __device__ __forceinline__ char* line_at(char* panels, int64_t row, int64_t kb, 
 
 // Source of an operand [rows, k]: element (r, k) at x[r * ld + k], or transposed at x[k * ld + r]. `left_out` (null or one target
 // per index along x's first axis): indices with a negative target are zeros. amax: per row the largest finite magnitude.
-int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax, hipStream_t s);
+int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax,
+             bool known, hipStream_t s);  // known: amax is there already
 
 // z = W x^T piece: A = W rows (classes v0 .. v0 + cols), B = x rows. stats: per 256 classes and row the maximum and the sum of
 // exp(z - maximum); zt: the target's logit, where it lies in the piece.
@@ -54,9 +55,14 @@ struct Gradient {
 };
 int32_t gradient(const Gradient& a, hipStream_t s);
 
+// The largest finite magnitude of every row of an operand (as pack takes it).
+int32_t row_amax(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, float* amax, hipStream_t s);
+
 // ---- few rows (lce_direct.hip): the streamed operand [rows, k] in fp32 against N columns held as planes
+constexpr int64_t kTripleRows = 64;  // up to here operands are bf16 triples, beyond them fp16 pairs, which take amax
 inline int64_t plane_bytes(int64_t rows, int64_t k) { return ceil_div64(rows, 32) * ceil_div64(k, 16) * 3072; }
-int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* to, hipStream_t s);
+int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, const float* amax, char* to, hipStream_t s);
+int64_t direct_rows(int64_t N);  // rows of the streamed operand that share an entry of the statistics
 
 struct Direct {
   const float* a;
@@ -65,7 +71,8 @@ struct Direct {
   int64_t N, v0;
   int parts;  // the walk along k cut into that many (x's gradient)
   const float *target, *lse;
-  float *stats, *zt;   // statistics: per 128 classes and row
+  const float *a_amax, *x_amax;  // pairs: of the streamed operand's rows, of the columns
+  float *stats, *zt;   // statistics: per direct_rows(N) classes and row
   float* dz;           // cotangents [N, rows], row stride dz_ld, or null
   int64_t dz_ld;
   char* dz_planes;     // or null
@@ -81,6 +88,7 @@ int32_t direct_dx(const Direct& p, bool kcontig, hipStream_t s);
 // out (by_d: [d * ld + v], else [v * ld + d]) = g / count * sum_n x[n, d] dz[n, v]; planes: x's columns along k = n
 struct Outer {
   const char* planes;
+  const float* x_amax;  // of x's columns (pairs), or null (triples)
   const float* dz;
   int64_t dz_ld, N, D, cols;
   float* out;

@@ -148,15 +148,20 @@ constexpr int64_t kManyRows = 512;
 
 int32_t few_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,
                      float* loss, float* lse, hipStream_t s) {
-  const int64_t tiles = ceil_div64(V, 128);
+  const int64_t tiles = ceil_div64(V, lce::direct_rows(N));
+  const bool scaled = N > lce::kTripleRows;
+  float* wa = lse + N + 1;
   Scratch w;
-  const int64_t xp = w.want(lce::plane_bytes(N, D)), st = w.want(8 * tiles * N), run = w.want(12 * N);
+  const int64_t xp = w.want(lce::plane_bytes(N, D)), st = w.want(8 * tiles * N), run = w.want(12 * N), xa = w.want(4 * N);
   int32_t rc = w.get();
-  if (rc || (rc = lce::planes(x, ldx, false, N, D, target, w.at(xp), s))) return rc;
+  if (rc) return rc;
+  if (scaled && ((rc = lce::row_amax(W, ldw, !transW, V, D, nullptr, wa, s)) || (rc = lce::row_amax(x, ldx, false, N, D, target, w.f(xa), s)))) return rc;
+  if ((rc = lce::planes(x, ldx, false, N, D, target, scaled ? w.f(xa) : nullptr, w.at(xp), s))) return rc;
   float *m = w.f(run), *l = m + N, *zt = l + N;
   lce::Direct a = {};
   a.a = W; a.lda = ldw; a.rows = V; a.k = D;
   a.planes = w.at(xp); a.N = N; a.parts = 1; a.target = target;
+  a.a_amax = wa; a.x_amax = w.f(xa);
   a.stats = w.f(st); a.zt = zt;
   if ((rc = lce::direct_stats(a, transW, s)) || (rc = join_stats(w.f(st), tiles, N, m, l, true, s))) return rc;
   hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(TPB), 0, s, N, V, target, m, l, zt, lse, loss);
@@ -168,19 +173,26 @@ int32_t few_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ld
                      const float* lse, const float* g, float* dx, float* dW, hipStream_t s) {
   int64_t piece = (24ll << 20) / N / 128 * 128;  // cotangents of a piece: 4 + 6 bytes each, 240 MiB
   if (piece > V) piece = V;
-  const int64_t groups = ceil_div64(D, 128) * ceil_div64(N, N <= 32 ? 32 : N <= 64 ? 64 : 128);
+  const int64_t groups = ceil_div64(D, lce::direct_rows(N)) * ceil_div64(N, N <= 32 ? 32 : N <= 64 ? 64 : 128);
+  const bool scaled = N > lce::kTripleRows;
   const int parts = cut(groups, 2 * ctx().cu_count, ceil_div64(piece, 256), 256);
   Scratch w;
   const int64_t xp = w.want(lce::plane_bytes(N, D)), xt = w.want(dW ? lce::plane_bytes(D, N) : 0), dz = w.want(dW ? 4 * N * piece : 0),
-                zp = w.want(dx ? lce::plane_bytes(N, piece) : 0), dxp = w.want(dx && parts > 1 ? 4 * parts * N * D : 0);
+                zp = w.want(dx ? lce::plane_bytes(N, piece) : 0), dxp = w.want(dx && parts > 1 ? 4 * parts * N * D : 0), xa = w.want(4 * N),
+                xta = w.want(4 * D);
   int32_t rc = w.get();
-  if (rc || (rc = lce::planes(x, ldx, false, N, D, target, w.at(xp), s))) return rc;
-  if (dW && (rc = lce::planes(x, ldx, true, D, N, target, w.at(xt), s))) return rc;
+  if (rc) return rc;
+  if (scaled && ((rc = lce::row_amax(x, ldx, false, N, D, target, w.f(xa), s)) ||
+                 (dW && (rc = lce::row_amax(x, ldx, true, D, N, target, w.f(xta), s)))))
+    return rc;
+  if ((rc = lce::planes(x, ldx, false, N, D, target, scaled ? w.f(xa) : nullptr, w.at(xp), s))) return rc;
+  if (dW && (rc = lce::planes(x, ldx, true, D, N, target, scaled ? w.f(xta) : nullptr, w.at(xt), s))) return rc;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     const int64_t cols = V - v0 < piece ? V - v0 : piece;
     lce::Direct a = {};
     a.a = W + (transW ? v0 * ldw : v0); a.lda = ldw; a.rows = cols; a.k = D;
     a.planes = w.at(xp); a.N = N; a.v0 = v0; a.parts = 1; a.target = target; a.lse = lse;
+    a.a_amax = lse + N + 1 + v0; a.x_amax = w.f(xa);
     a.dz = dW ? w.f(dz) : nullptr;
     a.dz_ld = cols;
     a.dz_planes = dx ? w.at(zp) : nullptr;
@@ -196,7 +208,7 @@ int32_t few_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ld
     }
     if (dW) {
       lce::Outer o = {};
-      o.planes = w.at(xt); o.dz = w.f(dz); o.dz_ld = cols; o.N = N; o.D = D; o.cols = cols;
+      o.planes = w.at(xt); o.x_amax = scaled ? w.f(xta) : nullptr; o.dz = w.f(dz); o.dz_ld = cols; o.N = N; o.D = D; o.cols = cols;
       o.out = transW ? dW + v0 * D : dW + v0;
       o.ld = transW ? D : V;
       o.g = g; o.count = lse + N;
@@ -221,16 +233,16 @@ int32_t many_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
                       float* loss, float* lse, hipStream_t s) {
   const int64_t piece = panel_columns(N, D, V, false), tiles = ceil_div64(piece, lce::kPanel);
   Scratch w;
-  const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N), wa = w.want(4 * piece),
+  const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N),
                 st = w.want(8 * tiles * N), run = w.want(12 * N);
   int32_t rc = w.get();
-  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), s))) return rc;
+  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), false, s))) return rc;
   float *m = w.f(run), *l = m + N, *zt = l + N;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     const int64_t cols = V - v0 < piece ? V - v0 : piece;
-    if ((rc = lce::pack(W + (transW ? v0 * ldw : v0), ldw, !transW, cols, D, nullptr, w.at(wp), w.f(wa), s))) return rc;
+    if ((rc = lce::pack(W + (transW ? v0 * ldw : v0), ldw, !transW, cols, D, nullptr, w.at(wp), lse + N + 1 + v0, false, s))) return rc;
     lce::Logits a = {};
-    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = w.f(wa); a.x_amax = w.f(xa); a.target = target;
+    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = lse + N + 1 + v0; a.x_amax = w.f(xa); a.target = target;
     a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
     a.stats = w.f(st); a.zt = zt;
     if ((rc = lce::logits_stats(a, s))) return rc;
@@ -247,20 +259,20 @@ int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
   const int64_t d_tiles = ceil_div64(D, lce::kPanel), cus = ctx().cu_count;
   const int parts = cut(rows / lce::kPanel * d_tiles, cus, ptiles, 16), w_parts = cut(ptiles * d_tiles, cus, rows / lce::kPanel, 16);
   Scratch w;
-  const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N), wa = w.want(4 * piece),
+  const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N),
                 xt = w.want(dW ? lce::panel_bytes(D, N) : 0), xta = w.want(4 * D), wt = w.want(dx ? lce::panel_bytes(D, piece) : 0), wta = w.want(4 * D),
                 p = w.want(dx ? rows * ptiles * lce::kPanel * 4 : 0), pt = w.want(dW ? rows * ptiles * lce::kPanel * 4 : 0),
                 ps = w.want(4 * ptiles * rows), pts = w.want(4 * rows / lce::kPanel * ptiles * lce::kPanel),
                 dxp = w.want(dx && parts > 1 ? 4 * parts * N * D : 0), dwp = w.want(dW && w_parts > 1 ? 4 * w_parts * piece * D : 0);
   int32_t rc = w.get();
-  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), s))) return rc;
-  if (dW && (rc = lce::pack(x, ldx, true, D, N, target, w.at(xt), w.f(xta), s))) return rc;
+  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), false, s))) return rc;
+  if (dW && (rc = lce::pack(x, ldx, true, D, N, target, w.at(xt), w.f(xta), false, s))) return rc;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     const int64_t cols = V - v0 < piece ? V - v0 : piece;
     const float* Wv = W + (transW ? v0 * ldw : v0);
-    if ((rc = lce::pack(Wv, ldw, !transW, cols, D, nullptr, w.at(wp), w.f(wa), s))) return rc;
+    if ((rc = lce::pack(Wv, ldw, !transW, cols, D, nullptr, w.at(wp), const_cast<float*>(lse) + N + 1 + v0, true, s))) return rc;
     lce::Logits a = {};
-    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = w.f(wa); a.x_amax = w.f(xa); a.target = target;
+    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = lse + N + 1 + v0; a.x_amax = w.f(xa); a.target = target;
     a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
     a.lse = lse;
     a.p = dx ? w.at(p) : nullptr;
@@ -272,7 +284,7 @@ int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
     q.g = g;
     q.count = lse + N;
     if (dx) {
-      if ((rc = lce::pack(Wv, ldw, transW, D, cols, nullptr, w.at(wt), w.f(wta), s))) return rc;
+      if ((rc = lce::pack(Wv, ldw, transW, D, cols, nullptr, w.at(wt), w.f(wta), false, s))) return rc;
       q.a = w.at(wt); q.b = a.p; q.a_amax = w.f(wta); q.b_shift = a.p_shift; q.b_shift_ld = rows;
       q.rows_a = D; q.rows_b = N; q.k = cols;
       q.out = parts > 1 ? w.f(dxp) : dx;

@@ -1354,7 +1354,7 @@ def linear_cross_entropy(x, weight, target):
         raise ValueError("linear_cross_entropy: empty operand")
     xs, ts = contiguous(x), contiguous(target)
     ws, trans, ldw, _ = _gemm_operand(weight)
-    loss, lse = Array.empty([1]), Array.empty([N + 1])
+    loss, lse = Array.empty([1]), Array.empty([N + 1 + V])
     L.call("endia_hip_linear_cross_entropy_fwd", N, D, V, xs.data_ptr(), D, trans, ws.data_ptr(), ldw, ts.data_ptr(), loss.data_ptr(),
            lse.data_ptr())
 

@@ -413,7 +413,8 @@ ENDIA_API int32_t endia_hip_mse_fwd_bwd(int64_t n, const float* pred, const floa
  *      left out: it counts neither in n nor in any gradient, whatever x holds there, and its dx is zero. n = 0 gives
  *      loss 0. A target that is no class (NaN, or V and above) makes the loss, and the gradients that the row takes part
  *      in, NaN.
- *      fwd: loss is one device float; lse receives N + 1 floats (lse per row, then n), which bwd takes.
+ *      fwd: loss is one device float; lse receives N + 1 + V floats (lse per row, then n, then the largest magnitude of each
+ *      class's weights where operands are scaled by it), which bwd takes together with the x and W that fwd saw.
  *      bwd: g is one device float, the cotangent of the loss. dx [N, D] and dW (in W's storage order, contiguous) are
  *      overwritten; either may be null. */
 ENDIA_API int32_t endia_hip_linear_cross_entropy_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW,
