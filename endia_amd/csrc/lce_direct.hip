@@ -10,9 +10,9 @@
 // nearly right has cotangents far below 1, and no one scale fits all of its classes.
 // The small operand (x, or the cotangents) is brought into operand order once ("planes").
 //
-// up to 32 rows of x (stream_few_kernel): a work-group takes 32 rows of the streamed operand, its four waves share k out among
-// them without a barrier and add up in LDS. More (stream_kernel): 128 rows, 32 per wave, against up to 128 columns, whose planes
-// the waves share through LDS; the next chunk of both operands travels while this one is multiplied.
+// stream_kernel: 128 rows of the streamed operand a work-group, 32 per wave, against up to 128 columns, whose planes the waves
+// share through LDS; the next chunk of both operands travels while this one is multiplied. stream_few_kernel, for few rows of x
+// and few classes: 32 rows a work-group, its four waves share k out among them without a barrier and add up in LDS.
 #include "linear_cross_entropy.h"
 
 #include <type_traits>
@@ -266,8 +266,13 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   constexpr int STAGE = CS * NB * step_bytes<Op>(), P = Op::PARTS;
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int64_t r0 = (int64_t)blockIdx.x * 128 + wave * 32;
-  const int n0 = blockIdx.y * NB * 32, part = blockIdx.z;
+  // Work-groups are dealt round-robin to the 8 XCDs: those that read the same 128 rows for different columns follow each other on
+  // one XCD, so that the rows come from memory once and then from its L2.
+  const int ntiles = (int)((p.N + NB * 32 - 1) / (NB * 32)), turn = blockIdx.x >> 3;
+  const int64_t group = (int64_t)(turn / ntiles) * 8 + (blockIdx.x & 7);
+  if (group * 128 >= p.rows) return;
+  const int64_t r0 = group * 128 + wave * 32;
+  const int n0 = turn % ntiles * NB * 32, part = blockIdx.y;
   const int steps = (int)((p.k + 15) / 16), chunks = (steps + CS - 1) / CS, per = (chunks + p.parts - 1) / p.parts;
   const int c0 = min(part * per, chunks), c1 = min(c0 + per, chunks);
   const int blocks = (int)((p.N + 31) / 32), first_block = n0 / 32;
@@ -350,7 +355,7 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
         const float mw = red[(w * NB * 32 + tid) * 2], lw = red[(w * NB * 32 + tid) * 2 + 1];
         sum += lw == 0.f ? 0.f : lw * __builtin_amdgcn_exp2f((mw - m) * kLog2e);
       }
-      *reinterpret_cast<float2*>(p.stats + ((int64_t)blockIdx.x * p.N + n0 + tid) * 2) = make_float2(m, sum);
+      *reinterpret_cast<float2*>(p.stats + (group * p.N + n0 + tid) * 2) = make_float2(m, sum);
     }
   } else {
 #pragma unroll
@@ -463,7 +468,7 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
 
 template <int NB, typename Op, int MODE>
 int32_t stream(const Direct& p, bool kcontig, bool vec, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div64(p.rows, 128), (unsigned)ceil_div64(p.N, NB * 32), (unsigned)p.parts);
+  const dim3 grid((unsigned)(ceil_div64(ceil_div64(p.rows, 128), 8) * 8 * ceil_div64(p.N, NB * 32)), (unsigned)p.parts);
   if (!kcontig) hipLaunchKernelGGL((stream_kernel<NB, Op, false, false, MODE>), grid, dim3(TPB), 0, s, p);
   else if (vec) hipLaunchKernelGGL((stream_kernel<NB, Op, true, true, MODE>), grid, dim3(TPB), 0, s, p);
   else hipLaunchKernelGGL((stream_kernel<NB, Op, true, false, MODE>), grid, dim3(TPB), 0, s, p);
@@ -471,12 +476,15 @@ int32_t stream(const Direct& p, bool kcontig, bool vec, hipStream_t s) {
   return ENDIA_HIP_OK;
 }
 
+// Up to 32 rows of x and so few classes that groups of 128 would leave half of the CUs idle: groups of 32.
+int64_t rows_per_group(int64_t N, int64_t rows) { return N <= 32 && ceil_div64(rows, 128) * 2 < endia::ctx().cu_count ? 32 : 128; }
+
 // Op: operands of statistics and cotangents beyond kTripleRows rows of x are pairs, all others triples
 template <int MODE>
 int32_t stream(const Direct& p, bool kcontig, hipStream_t s) {
   using Op = typename std::conditional<MODE == DX, Triple, Pair>::type;
   const bool vec = kcontig && p.lda % 4 == 0 && p.k % 4 == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
-  if (p.N <= 32) {
+  if (MODE != DX && rows_per_group(p.N, p.rows) == 32) {
     const dim3 grid((unsigned)ceil_div64(p.rows, 32), 1, (unsigned)p.parts);
     if (!kcontig) hipLaunchKernelGGL((stream_few_kernel<false, false, MODE>), grid, dim3(TPB), 0, s, p);
     else if (vec) hipLaunchKernelGGL((stream_few_kernel<true, true, MODE>), grid, dim3(TPB), 0, s, p);
@@ -484,6 +492,7 @@ int32_t stream(const Direct& p, bool kcontig, hipStream_t s) {
     ENDIA_LAUNCH_CHECK();
     return ENDIA_HIP_OK;
   }
+  if (p.N <= 32) return stream<1, Triple, MODE>(p, kcontig, vec, s);
   if (p.N <= kTripleRows) return stream<2, Triple, MODE>(p, kcontig, vec, s);
   // 96 or 128 columns at a time, whichever leaves fewer of them empty
   const int64_t blocks = ceil_div64(p.N, 32);
@@ -502,7 +511,7 @@ int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_
   return ENDIA_HIP_OK;
 }
 
-int64_t direct_rows(int64_t N) { return N <= 32 ? 32 : 128; }
+int64_t direct_rows(int64_t N, int64_t rows) { return rows_per_group(N, rows); }
 int32_t direct_stats(const Direct& p, bool kcontig, hipStream_t s) { return stream<STATS>(p, kcontig, s); }
 int32_t direct_dz(const Direct& p, bool kcontig, hipStream_t s) { return stream<DZ>(p, kcontig, s); }
 int32_t direct_dx(const Direct& p, bool kcontig, hipStream_t s) { return stream<DX>(p, kcontig, s); }

@@ -62,7 +62,7 @@ int32_t row_amax(const float* x, int64_t ld, bool transposed, int64_t rows, int6
 constexpr int64_t kTripleRows = 64;  // up to here operands are bf16 triples, beyond them fp16 pairs, which take amax
 inline int64_t plane_bytes(int64_t rows, int64_t k) { return ceil_div64(rows, 32) * ceil_div64(k, 16) * 3072; }
 int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, const float* amax, char* to, hipStream_t s);
-int64_t direct_rows(int64_t N);  // rows of the streamed operand that share an entry of the statistics
+int64_t direct_rows(int64_t N, int64_t rows);  // rows of the streamed operand that share an entry of the statistics
 
 struct Direct {
   const float* a;
@@ -72,7 +72,7 @@ struct Direct {
   int parts;  // the walk along k cut into that many (x's gradient)
   const float *target, *lse;
   const float *a_amax, *x_amax;  // pairs: of the streamed operand's rows, of the columns
-  float *stats, *zt;   // statistics: per direct_rows(N) classes and row
+  float *stats, *zt;   // statistics: per direct_rows(N, rows) classes and row
   float* dz;           // cotangents [N, rows], row stride dz_ld, or null
   int64_t dz_ld;
   char* dz_planes;     // or null

@@ -148,7 +148,7 @@ constexpr int64_t kManyRows = 512;
 
 int32_t few_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,
                      float* loss, float* lse, hipStream_t s) {
-  const int64_t tiles = ceil_div64(V, lce::direct_rows(N));
+  const int64_t tiles = ceil_div64(V, lce::direct_rows(N, V));
   const bool scaled = N > lce::kTripleRows;
   float* wa = lse + N + 1;
   Scratch w;
@@ -173,7 +173,7 @@ int32_t few_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ld
                      const float* lse, const float* g, float* dx, float* dW, hipStream_t s) {
   int64_t piece = (24ll << 20) / N / 128 * 128;  // cotangents of a piece: 4 + 6 bytes each, 240 MiB
   if (piece > V) piece = V;
-  const int64_t groups = ceil_div64(D, lce::direct_rows(N)) * ceil_div64(N, N <= 32 ? 32 : N <= 64 ? 64 : 128);
+  const int64_t groups = ceil_div64(D, 128) * ceil_div64(N, N <= 32 ? 32 : N <= 64 ? 64 : 128);
   const bool scaled = N > lce::kTripleRows;
   const int parts = cut(groups, 2 * ctx().cu_count, ceil_div64(piece, 256), 256);
   Scratch w;
