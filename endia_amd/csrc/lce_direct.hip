@@ -82,24 +82,25 @@ __device__ __forceinline__ floatx16 multiply(const Triple& a, const Triple& b, f
 // accumulator holds its rows, so that cotangents become operands as they lie.
 __device__ __forceinline__ int k_of(int half, int e) { return 8 * (e >> 2) + 4 * half + (e & 3); }
 
-// Elements k0 + k_of(half, e) of row r of an operand that lies contiguous along k (x[r * ld + k]) or along r (x[k * ld + r]). Loads
-// go out unconditionally, clamped to the operand; what lies behind its end becomes zero.
-template <bool KCONTIG, bool VEC>
+// Elements k0 + k_of(half, e) of row r of an operand that lies contiguous along k (x[r * ld + k]: 16 bytes at a time, which global
+// memory gives from any multiple of 4) or along r (x[k * ld + r]). Rows behind the operand's end read its last one; what lies
+// behind the end of k becomes zero.
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+template <bool KCONTIG>
 __device__ __forceinline__ void load_step(const float* __restrict__ x, int64_t ld, int64_t r, int64_t rows, int64_t k0, int64_t k, int half, float (&v)[8]) {
   r = min(r, rows - 1);
-  if (KCONTIG && VEC) {
+  if (KCONTIG && k0 + 16 <= k) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int64_t at = k0 + 8 * j + 4 * half;
-      const float4 f = *reinterpret_cast<const float4*>(x + r * ld + min(at, k - 4));
-      v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+      const float4u f = *reinterpret_cast<const float4u*>(x + r * ld + k0 + 8 * j + 4 * half);
+      v[4 * j] = f[0]; v[4 * j + 1] = f[1]; v[4 * j + 2] = f[2]; v[4 * j + 3] = f[3];
     }
-  } else {
+    return;
+  }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t at = min(k0 + k_of(half, e), k - 1);
-      v[e] = KCONTIG ? x[r * ld + at] : x[at * ld + r];
-    }
+  for (int e = 0; e < 8; ++e) {
+    const int64_t at = min(k0 + k_of(half, e), k - 1);
+    v[e] = KCONTIG ? x[r * ld + at] : x[at * ld + r];
   }
   if (k0 + 16 > k) {
 #pragma unroll
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(TPB) void planes_kernel(const float* __restrict__ x
   const int64_t steps = (k + 15) / 16, step = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), block = blockIdx.y, r = block * 32 + (lane & 31);
   if (step >= steps) return;
   float v[8];
-  load_step<KCONTIG, false>(x, ld, r, rows, step * 16, k, half, v);
+  load_step<KCONTIG>(x, ld, r, rows, step * 16, k, half, v);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int64_t i = KCONTIG ? r : step * 16 + k_of(half, e);  // index along x's first axis
@@ -206,7 +207,7 @@ __device__ __forceinline__ void dx_block(const Direct& p, const floatx16& acc, i
 }
 
 // Up to 32 rows of x. Waves take chunks of 4 steps in turn; nothing is shared until the end.
-template <bool KCONTIG, bool VEC, int MODE>
+template <bool KCONTIG, int MODE>
 __global__ __launch_bounds__(TPB, 2) void stream_few_kernel(Direct p) {
   constexpr int CS = 4;
   __shared__ float red[4][16][64];
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(TPB, 2) void stream_few_kernel(Direct p) {
   auto fetch = [&](int c) {
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
-      load_step<KCONTIG, VEC>(p.a, p.lda, r0 + col, p.rows, (int64_t)(c * CS + s) * 16, p.k, half, next[s]);
+      load_step<KCONTIG>(p.a, p.lda, r0 + col, p.rows, (int64_t)(c * CS + s) * 16, p.k, half, next[s]);
       xn[s] = read_planes<Triple>(p.planes + (int64_t)min(c * CS + s, steps - 1) * step_bytes<Triple>(), lane);
     }
   };
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(TPB, 2) void stream_few_kernel(Direct p) {
   }
 }
 
-template <int NB, typename Op, bool KCONTIG, bool VEC, int MODE>
+template <int NB, typename Op, bool KCONTIG, int MODE>
 __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   constexpr int CS = NB > 2 ? 2 : 4;  // steps per chunk
   constexpr int STAGE = CS * NB * step_bytes<Op>(), P = Op::PARTS;
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   float next[CS][8], now[CS][8];
   auto fetch = [&](int c) {
 #pragma unroll
-    for (int s = 0; s < CS; ++s) load_step<KCONTIG, VEC>(p.a, p.lda, r0 + col, p.rows, (int64_t)(c * CS + s) * 16, p.k, half, next[s]);
+    for (int s = 0; s < CS; ++s) load_step<KCONTIG>(p.a, p.lda, r0 + col, p.rows, (int64_t)(c * CS + s) * 16, p.k, half, next[s]);
   };
   floatx16 acc[NB];
 #pragma unroll
@@ -366,11 +367,11 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   }
 }
 
-// dW[d, v] = c sum_n x[n, d] dz[n, v]: a wave takes 32 classes against 4 x 32 of x's columns at a time, whose planes the four waves
-// share through LDS. Bound: HBM (the gradient is written once) up to about 128 rows.
+// dW[d, v] = c sum_n x[n, d] dz[n, v]: a wave takes 32 classes against 4 x 32 (pairs: 8 x 32) of x's columns at a time, whose planes
+// the four waves share through LDS. Bound: HBM (the gradient is written once) up to about 128 rows.
 template <bool BY_D, typename Op>
 __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
-  constexpr int DB = 4, CS = 2, P = Op::PARTS, STAGE = DB * CS * step_bytes<Op>();
+  constexpr int P = Op::PARTS, DB = P == 2 ? 8 : 4, CS = 2, STAGE = DB * CS * step_bytes<Op>();
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int64_t v0 = (int64_t)blockIdx.x * 128 + wave * 32, v = v0 + col;
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
   auto fetch = [&](int turn) {
     const int ch = turn % chunks;
 #pragma unroll
-    for (int s = 0; s < CS; ++s) load_step<false, false>(p.dz, p.dz_ld, v, p.cols, (int64_t)(ch * CS + s) * 16, p.N, half, next[s]);
+    for (int s = 0; s < CS; ++s) load_step<false>(p.dz, p.dz_ld, v, p.cols, (int64_t)(ch * CS + s) * 16, p.N, half, next[s]);
   };
   floatx16 acc[DB];
 #pragma unroll
@@ -433,31 +434,27 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
     }
     if (turn % chunks == chunks - 1) {
       const int d0 = (g0 + turn / chunks) * DB * 32;
-      // the axis that lies contiguous in the output is the one along the lanes
-      if (P == 2) {
-        const float down_v = __builtin_ldexpf(1.f, -shift);  // of the lane's class: with classes along the registers, lane k has theirs
+      // The axis that lies contiguous in the output is the one along the lanes. (Pairs: the scales come off, of the lane's class and
+      // of x's columns; with classes along the registers, lane k has those of class k.)
+      const float down_v = P == 2 ? __builtin_ldexpf(c, -shift) : c;
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int k = k_of(half, i & 7) + 16 * (i >> 3), d = d0 + b * 32 + (BY_D ? k : col);
-            const float down_x = __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min(d, (int)p.D - 1)]));
-            acc[b][i] *= down_x * (BY_D ? down_v : __shfl(down_v, k, 64));
-          }
-      }
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
+      for (int b = 0; b < DB; ++b) {
+        const float down_lane = P == 2 && !BY_D ? __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min(d0 + b * 32 + col, (int)p.D - 1)])) : 1.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int k = k_of(half, i & 7) + 16 * (i >> 3);
           if (BY_D) {
             const int d = d0 + b * 32 + k;
-            if (v < p.cols && d < p.D) p.out[(int64_t)d * p.ld + v] = acc[b][i] * c;
+            const float down = P == 2 ? __builtin_ldexpf(down_v, -pairs::shift_of(p.x_amax[min(d, (int)p.D - 1)])) : down_v;
+            if (v < p.cols && d < p.D) p.out[(int64_t)d * p.ld + v] = acc[b][i] * down;
           } else {
             const int d = d0 + b * 32 + col;
-            if (d < p.D && v0 + k < p.cols) p.out[(v0 + k) * p.ld + d] = acc[b][i] * c;
+            const float down = P == 2 ? down_lane * __shfl(down_v, k, 64) : c;
+            if (d < p.D && v0 + k < p.cols) p.out[(v0 + k) * p.ld + d] = acc[b][i] * down;
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int b = 0; b < DB; ++b) acc[b] = floatx16{};
     }
@@ -467,11 +464,10 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
 }
 
 template <int NB, typename Op, int MODE>
-int32_t stream(const Direct& p, bool kcontig, bool vec, hipStream_t s) {
+int32_t stream_tiles(const Direct& p, bool kcontig, hipStream_t s) {
   const dim3 grid((unsigned)(ceil_div64(ceil_div64(p.rows, 128), 8) * 8 * ceil_div64(p.N, NB * 32)), (unsigned)p.parts);
-  if (!kcontig) hipLaunchKernelGGL((stream_kernel<NB, Op, false, false, MODE>), grid, dim3(TPB), 0, s, p);
-  else if (vec) hipLaunchKernelGGL((stream_kernel<NB, Op, true, true, MODE>), grid, dim3(TPB), 0, s, p);
-  else hipLaunchKernelGGL((stream_kernel<NB, Op, true, false, MODE>), grid, dim3(TPB), 0, s, p);
+  if (kcontig) hipLaunchKernelGGL((stream_kernel<NB, Op, true, MODE>), grid, dim3(TPB), 0, s, p);
+  else hipLaunchKernelGGL((stream_kernel<NB, Op, false, MODE>), grid, dim3(TPB), 0, s, p);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }
@@ -483,20 +479,18 @@ int64_t rows_per_group(int64_t N, int64_t rows) { return N <= 32 && ceil_div64(r
 template <int MODE>
 int32_t stream(const Direct& p, bool kcontig, hipStream_t s) {
   using Op = typename std::conditional<MODE == DX, Triple, Pair>::type;
-  const bool vec = kcontig && p.lda % 4 == 0 && p.k % 4 == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
   if (MODE != DX && rows_per_group(p.N, p.rows) == 32) {
     const dim3 grid((unsigned)ceil_div64(p.rows, 32), 1, (unsigned)p.parts);
-    if (!kcontig) hipLaunchKernelGGL((stream_few_kernel<false, false, MODE>), grid, dim3(TPB), 0, s, p);
-    else if (vec) hipLaunchKernelGGL((stream_few_kernel<true, true, MODE>), grid, dim3(TPB), 0, s, p);
-    else hipLaunchKernelGGL((stream_few_kernel<true, false, MODE>), grid, dim3(TPB), 0, s, p);
+    if (kcontig) hipLaunchKernelGGL((stream_few_kernel<true, MODE>), grid, dim3(TPB), 0, s, p);
+    else hipLaunchKernelGGL((stream_few_kernel<false, MODE>), grid, dim3(TPB), 0, s, p);
     ENDIA_LAUNCH_CHECK();
     return ENDIA_HIP_OK;
   }
-  if (p.N <= 32) return stream<1, Triple, MODE>(p, kcontig, vec, s);
-  if (p.N <= kTripleRows) return stream<2, Triple, MODE>(p, kcontig, vec, s);
+  if (p.N <= 32) return stream_tiles<1, Triple, MODE>(p, kcontig, s);
+  if (p.N <= kTripleRows) return stream_tiles<2, Triple, MODE>(p, kcontig, s);
   // 96 or 128 columns at a time, whichever leaves fewer of them empty
   const int64_t blocks = ceil_div64(p.N, 32);
-  return ceil_div64(blocks, 3) * 3 < ceil_div64(blocks, 4) * 4 ? stream<3, Op, MODE>(p, kcontig, vec, s) : stream<4, Op, MODE>(p, kcontig, vec, s);
+  return ceil_div64(blocks, 3) * 3 < ceil_div64(blocks, 4) * 4 ? stream_tiles<3, Op, MODE>(p, kcontig, s) : stream_tiles<4, Op, MODE>(p, kcontig, s);
 }
 
 }  // namespace
@@ -518,7 +512,7 @@ int32_t direct_dx(const Direct& p, bool kcontig, hipStream_t s) { return stream<
 
 int32_t direct_dw(const Outer& q, bool by_d, hipStream_t s) {
   Outer p = q;
-  const int64_t vg = ceil_div64(p.cols, 128), groups = ceil_div64(p.D, 128);
+  const int64_t vg = ceil_div64(p.cols, 128), groups = ceil_div64(p.D, p.x_amax ? 256 : 128);
   int64_t cuts = ceil_div64(4 * endia::ctx().cu_count, vg);  // work-groups along x's columns, when the classes alone do not fill the chip
   if (cuts > groups) cuts = groups;
   p.groups = (int)ceil_div64(groups, cuts);

@@ -9,6 +9,7 @@ namespace {
 
 using namespace pairs;
 constexpr int TPB = 256;
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ void store_chunk(char* line, int row, int chunk, const float (&v)[8], int shift) {
   float y[8];
@@ -21,7 +22,6 @@ __device__ __forceinline__ void store_chunk(char* line, int row, int chunk, cons
 }
 
 // Source rows contiguous along k: one wave per row, the row twice (the second time from cache).
-template <bool VEC>
 __global__ __launch_bounds__(TPB) void pack_rows_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, const float* __restrict__ left_out,
                                                         char* __restrict__ panels, float* __restrict__ amax_out, int known) {
   const int lane = threadIdx.x & 63;
@@ -31,12 +31,11 @@ __global__ __launch_bounds__(TPB) void pack_rows_kernel(const float* __restrict_
   const float* r = x + row * ld;
   float amax = 0.f;
   auto load8 = [&](int64_t k0, float (&v)[8]) {
-    if (VEC) {
+    if (k0 + 8 <= k) {  // (global memory gives 16 bytes from any multiple of 4)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int64_t at = k0 + 4 * j;
-        const float4 f = at < k ? *reinterpret_cast<const float4*>(r + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+        const float4u f = *reinterpret_cast<const float4u*>(r + k0 + 4 * j);
+        v[4 * j] = f[0]; v[4 * j + 1] = f[1]; v[4 * j + 2] = f[2]; v[4 * j + 3] = f[3];
       }
     } else {
 #pragma unroll
@@ -129,10 +128,7 @@ int32_t row_amax(const float* x, int64_t ld, bool transposed, int64_t rows, int6
 int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax, bool known,
              hipStream_t s) {
   if (!transposed) {
-    const bool vec = k % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    const dim3 grid((unsigned)ceil_div64(rows, 4));
-    if (vec) hipLaunchKernelGGL(pack_rows_kernel<true>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax, known ? 1 : 0);
-    else hipLaunchKernelGGL(pack_rows_kernel<false>, grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax, known ? 1 : 0);
+    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)ceil_div64(rows, 4)), dim3(TPB), 0, s, x, ld, rows, k, left_out, panels, amax, known ? 1 : 0);
     ENDIA_LAUNCH_CHECK();
     return ENDIA_HIP_OK;
   }

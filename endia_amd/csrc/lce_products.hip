@@ -16,30 +16,40 @@ namespace lce {
 namespace {
 
 using namespace pairs;
-constexpr int TPB = 512, FA = 4, FB = 2;  // blocks of 32 x 32 per wave
-constexpr int STAGE = 2 * kPanel * 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// T x T of C: 256 (8 waves, 2 x 4, of 128 x 64) or 128 (4 waves, 2 x 2, of 64 x 64, two work-groups per CU)
+template <int T>
 struct Tile {
-  int lane, wave, col, half, wa, wb;  // wa: wave along a (2), wb: along b (4)
+  static constexpr int TPB = T == 256 ? 512 : 256, WB = T == 256 ? 4 : 2, FA = T == 256 ? 4 : 2, FB = 2;  // FA x FB blocks of 32 x 32 per wave
+  static constexpr int STAGE = 2 * T * 128, PER_PANEL = kPanel / T;
+  typedef floatx16 Acc[FA][FB];
+  int lane, wave, col, half, wa, wb;  // the wave's place along a and b
   __device__ __forceinline__ Tile() {
     lane = threadIdx.x & 63;
     wave = threadIdx.x >> 6;
     col = lane & 31;
     half = lane >> 5;
-    wa = wave >> 2;
-    wb = wave & 3;
+    wa = wave / WB;
+    wb = wave % WB;
   }
-  __device__ __forceinline__ int a_of(int fa, int v) const { return wa * 128 + fa * 32 + 8 * (v >> 2) + 4 * half + (v & 3); }
-  __device__ __forceinline__ int b_of(int fb) const { return wb * 64 + fb * 32 + col; }
+  __device__ __forceinline__ int a_of(int fa, int v) const { return wa * FA * 32 + fa * 32 + 8 * (v >> 2) + 4 * half + (v & 3); }
+  __device__ __forceinline__ int b_of(int fb) const { return wb * FB * 32 + fb * 32 + col; }
+  // block 0 of k of tile t (a panel of 256 rows holds PER_PANEL tiles)
+  __device__ __forceinline__ static const char* panel(const char* x, int t, int64_t kblocks) {
+    return x + (t / PER_PANEL) * kblocks * kBlockBytes + t % PER_PANEL * T * 128;
+  }
 };
+typedef Tile<256> Tile256;
+constexpr int FA = Tile256::FA, FB = Tile256::FB, TPB = Tile256::TPB, STAGE = Tile256::STAGE;
 
-__device__ __forceinline__ void request(const char* a, const char* b, char* stage, const Tile& t) {
+template <int T>
+__device__ __forceinline__ void request(const char* a, const char* b, char* stage, const Tile<T>& t) {
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    const int at = (p * 8 + t.wave) * 1024;
+    const int at = (p * (Tile<T>::TPB / 64) + t.wave) * 1024;
     load_to_lds(a + at + t.lane * 16, stage + at);
-    load_to_lds(b + at + t.lane * 16, stage + STAGE / 2 + at);
+    load_to_lds(b + at + t.lane * 16, stage + Tile<T>::STAGE / 2 + at);
   }
 }
 
@@ -49,8 +59,10 @@ __device__ __forceinline__ void read_line(const char* lines, int line, int s, in
   lo = *reinterpret_cast<const half8*>(at + (((4 + 2 * s + h) ^ (line & 7)) << 4));
 }
 
-__device__ __forceinline__ void multiply(const char* stage, const Tile& t, floatx16 (&acc)[FA][FB]) {
-  const char *sa = stage + t.wa * 128 * 128, *sb = stage + STAGE / 2 + t.wb * 64 * 128;
+template <int T>
+__device__ __forceinline__ void multiply(const char* stage, const Tile<T>& t, typename Tile<T>::Acc& acc) {
+  constexpr int FA = Tile<T>::FA, FB = Tile<T>::FB;
+  const char *sa = stage + t.wa * FA * 32 * 128, *sb = stage + Tile<T>::STAGE / 2 + t.wb * FB * 32 * 128;
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
     half8 ah[FA], al[FA], bh[FB], bl[FB];
@@ -70,26 +82,29 @@ __device__ __forceinline__ void multiply(const char* stage, const Tile& t, float
   }
 }
 
-__device__ __forceinline__ void clear(floatx16 (&acc)[FA][FB]) {
+template <int T>
+__device__ __forceinline__ void clear(typename Tile<T>::Acc& acc) {
 #pragma unroll
-  for (int i = 0; i < FA; ++i)
+  for (int i = 0; i < Tile<T>::FA; ++i)
 #pragma unroll
-    for (int j = 0; j < FB; ++j) acc[i][j] = floatx16{};
+    for (int j = 0; j < Tile<T>::FB; ++j) acc[i][j] = floatx16{};
 }
 
 // z in place of the accumulator: the scales of both operands come off (classes behind the piece's end become -inf). The factors
-// wait in LDS (512 floats at `lds`).
-__device__ __forceinline__ void to_logits(const Logits& p, const Tile& t, int64_t a0, int64_t b0, float* lds, floatx16 (&acc)[FA][FB]) {
+// wait in LDS (2 T floats at `lds`).
+template <int T>
+__device__ __forceinline__ void to_logits(const Logits& p, const Tile<T>& t, int64_t a0, int64_t b0, float* lds, typename Tile<T>::Acc& acc) {
+  constexpr int FA = Tile<T>::FA, FB = Tile<T>::FB;
   {
-    const int i = threadIdx.x & (kPanel - 1);
-    const float amax = threadIdx.x < kPanel ? p.w_amax[min(a0 + i, p.cols - 1)] : p.x_amax[min(b0 + i, p.N - 1)];
+    const int i = threadIdx.x & (T - 1);
+    const float amax = threadIdx.x < T ? p.w_amax[min(a0 + i, p.cols - 1)] : p.x_amax[min(b0 + i, p.N - 1)];
     lds[threadIdx.x] = __builtin_ldexpf(1.f, -shift_of(amax));
   }
   __syncthreads();
   float cb[FB];
 #pragma unroll
-  for (int j = 0; j < FB; ++j) cb[j] = lds[kPanel + t.b_of(j)];
-  const int left = (int)min(p.cols - a0, (int64_t)kPanel);
+  for (int j = 0; j < FB; ++j) cb[j] = lds[T + t.b_of(j)];
+  const int left = (int)min(p.cols - a0, (int64_t)T);
 #pragma unroll
   for (int i = 0; i < FA; ++i) {
 #pragma unroll
@@ -98,7 +113,7 @@ __device__ __forceinline__ void to_logits(const Logits& p, const Tile& t, int64_
 #pragma unroll
       for (int j = 0; j < FB; ++j) acc[i][j][v] = acc[i][j][v] * ca * cb[j];
     }
-    if (left < kPanel) {
+    if (left < T) {
 #pragma unroll
       for (int v = 0; v < 16; ++v)
 #pragma unroll
@@ -108,10 +123,12 @@ __device__ __forceinline__ void to_logits(const Logits& p, const Tile& t, int64_
   }
 }
 
-__device__ __forceinline__ void logits_tile(const Logits& p, const Tile& t, int ta, int tb, char* smem, floatx16 (&acc)[FA][FB]) {
+template <int T>
+__device__ __forceinline__ void logits_tile(const Logits& p, const Tile<T>& t, int ta, int tb, char* smem, typename Tile<T>::Acc& acc) {
+  constexpr int STAGE = Tile<T>::STAGE;
   const int kblocks = (int)((p.D + kBlock - 1) / kBlock);
-  const char *a = p.w + (int64_t)ta * kblocks * kBlockBytes, *b = p.x + (int64_t)tb * kblocks * kBlockBytes;
-  clear(acc);
+  const char *a = t.panel(p.w, ta, kblocks), *b = t.panel(p.x, tb, kblocks);
+  clear<T>(acc);
   request(a, b, smem, t);
   wait_loads();
   __syncthreads();
@@ -123,17 +140,19 @@ __device__ __forceinline__ void logits_tile(const Logits& p, const Tile& t, int 
   }
 }
 
-__global__ __launch_bounds__(TPB, 2) void stats_kernel(Logits p) {
+template <int T>
+__global__ __launch_bounds__(Tile<T>::TPB, 2) void stats_kernel(Logits p) {
+  constexpr int FA = Tile<T>::FA, FB = Tile<T>::FB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const Tile t;
+  const Tile<T> t;
   int ta, tb;
-  const int tiles_a = (int)((p.cols + kPanel - 1) / kPanel), tiles_b = (int)((p.N + kPanel - 1) / kPanel);
+  const int tiles_a = (int)((p.cols + T - 1) / T), tiles_b = (int)((p.N + T - 1) / T);
   mfma::tile_of_block(blockIdx.x, gridDim.x, tiles_a, tiles_b, ta, tb);
-  floatx16 acc[FA][FB];
+  typename Tile<T>::Acc acc;
   logits_tile(p, t, ta, tb, smem, acc);
-  const int64_t a0 = (int64_t)ta * kPanel, b0 = (int64_t)tb * kPanel;
-  to_logits(p, t, a0, b0, reinterpret_cast<float*>(smem) + 4 * kPanel, acc);
-  float* red = reinterpret_cast<float*>(smem);  // [2 (wa)][256 rows of x][2]
+  const int64_t a0 = (int64_t)ta * T, b0 = (int64_t)tb * T;
+  to_logits(p, t, a0, b0, reinterpret_cast<float*>(smem) + 4 * T, acc);
+  float* red = reinterpret_cast<float*>(smem);  // [2 (wa)][T rows of x][2]
 #pragma unroll
   for (int j = 0; j < FB; ++j) {
     const int64_t n = b0 + t.b_of(j);
@@ -155,7 +174,7 @@ __global__ __launch_bounds__(TPB, 2) void stats_kernel(Logits p) {
       }
     sum += __shfl_xor(sum, 32, 64);
     const float local = target - (float)(p.v0 + a0);
-    if (local >= 0.f && local < (float)kPanel) {
+    if (local >= 0.f && local < (float)T) {
 #pragma unroll
       for (int i = 0; i < FA; ++i)
 #pragma unroll
@@ -163,14 +182,14 @@ __global__ __launch_bounds__(TPB, 2) void stats_kernel(Logits p) {
           if ((int)local == t.a_of(i, v)) p.zt[n] = acc[i][j][v];
     }
     if (t.half == 0) {
-      red[(t.wa * kPanel + t.b_of(j)) * 2] = m;
-      red[(t.wa * kPanel + t.b_of(j)) * 2 + 1] = sum;
+      red[(t.wa * T + t.b_of(j)) * 2] = m;
+      red[(t.wa * T + t.b_of(j)) * 2 + 1] = sum;
     }
   }
   __syncthreads();
   const int64_t n = b0 + threadIdx.x;
-  if (threadIdx.x < kPanel && n < p.N) {
-    const float m0 = red[threadIdx.x * 2], l0 = red[threadIdx.x * 2 + 1], m1 = red[(kPanel + threadIdx.x) * 2], l1 = red[(kPanel + threadIdx.x) * 2 + 1];
+  if (threadIdx.x < T && n < p.N) {
+    const float m0 = red[threadIdx.x * 2], l0 = red[threadIdx.x * 2 + 1], m1 = red[(T + threadIdx.x) * 2], l1 = red[(T + threadIdx.x) * 2 + 1];
     const float m = fmaxf(m0, m1);
     const float w0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m0 - m) * kLog2e), w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m1 - m) * kLog2e);
     float* to = p.stats + ((int64_t)ta * p.N + n) * 2;
@@ -185,7 +204,7 @@ __global__ __launch_bounds__(TPB, 2) void stats_kernel(Logits p) {
 // tile's own largest, so that rows that are nearly right and classes that are hardly likely keep their precision.
 __global__ __launch_bounds__(TPB, 2) void dz_kernel(Logits p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const Tile t;
+  const Tile256 t;
   int ta, tb;
   const int tiles_a = (int)((p.cols + kPanel - 1) / kPanel), tiles_b = (int)((p.N + kPanel - 1) / kPanel);
   mfma::tile_of_block(blockIdx.x, gridDim.x, tiles_a, tiles_b, ta, tb);
@@ -320,20 +339,22 @@ __global__ __launch_bounds__(TPB, 2) void dz_kernel(Logits p) {
   }
 }
 
-__global__ __launch_bounds__(TPB, 2) void gradient_kernel(Gradient p) {
+template <int T>
+__global__ __launch_bounds__(Tile<T>::TPB, 2) void gradient_kernel(Gradient p) {
+  constexpr int FA = Tile<T>::FA, FB = Tile<T>::FB, STAGE = Tile<T>::STAGE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const Tile t;
-  const int tiles_a = (int)((p.rows_a + kPanel - 1) / kPanel), tiles_b = (int)((p.rows_b + kPanel - 1) / kPanel), tiles = tiles_a * tiles_b;
+  const Tile<T> t;
+  const int tiles_a = (int)((p.rows_a + T - 1) / T), tiles_b = (int)((p.rows_b + T - 1) / T), tiles = tiles_a * tiles_b;
   const int part = blockIdx.x / tiles;
   int ta, tb;
   mfma::tile_of_block(blockIdx.x % tiles, tiles, tiles_a, tiles_b, ta, tb);
   const int kblocks = (int)((p.k + kBlock - 1) / kBlock), panels = (kblocks + 7) / 8;
   const int64_t b_blocks = (int64_t)panels * 8;  // b was written in whole panels of k
   const int per = (panels + p.parts - 1) / p.parts, k0 = min(part * per * 8, kblocks), k1 = min(k0 + per * 8, kblocks);
-  const char *a = p.a + (int64_t)ta * kblocks * kBlockBytes, *b = p.b + (int64_t)tb * b_blocks * kBlockBytes;
-  const int64_t a0 = (int64_t)ta * kPanel, b0 = (int64_t)tb * kPanel;
-  floatx16 acc[FA][FB];
-  clear(acc);
+  const char *a = t.panel(p.a, ta, kblocks), *b = t.panel(p.b, tb, b_blocks);
+  const int64_t a0 = (int64_t)ta * T, b0 = (int64_t)tb * T;
+  typename Tile<T>::Acc acc;
+  clear<T>(acc);
   int shift[FB];
   const int* shifts = p.b_shift + b0;
 #pragma unroll
@@ -397,22 +418,37 @@ __global__ __launch_bounds__(TPB, 2) void gradient_kernel(Gradient p) {
   }
 }
 
-template <typename Kernel, typename Params>
+template <int T, typename Kernel, typename Params>
 int32_t launch(Kernel* kernel, const Params& p, int64_t groups, hipStream_t s) {
-  ENDIA_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(TPB), 2 * STAGE, s, p);
+  constexpr int lds = 2 * Tile<T>::STAGE;
+  ENDIA_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(Tile<T>::TPB), lds, s, p);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }
 
+// 256 x 256 tiles run at the higher rate, 128 x 128 ones (two to a CU, about three quarters of the rate) waste less of the last
+// round and of ragged edges: whichever takes fewer rounds of the chip, in units of a quarter tile.
+int64_t tiles_of(int64_t a, int64_t b, int T) { return ceil_div64(a, T) * ceil_div64(b, T); }
+
 }  // namespace
 
-int32_t logits_stats(const Logits& p, hipStream_t s) { return launch(stats_kernel, p, ceil_div64(p.cols, kPanel) * ceil_div64(p.N, kPanel), s); }
-int32_t logits_dz(const Logits& p, hipStream_t s) { return launch(dz_kernel, p, ceil_div64(p.cols, kPanel) * ceil_div64(p.N, kPanel), s); }
+int product_tile(int64_t a, int64_t b) {
+  const int64_t cus = endia::ctx().cu_count;
+  const int64_t big = ceil_div64(tiles_of(a, b, 256), cus) * 4 * 3, small = ceil_div64(tiles_of(a, b, 128), 2 * cus) * 2 * 4;
+  return small < big ? 128 : 256;
+}
+
+int32_t logits_stats(const Logits& p, hipStream_t s) {
+  return product_tile(p.cols, p.N) == 256 ? launch<256>(stats_kernel<256>, p, tiles_of(p.cols, p.N, 256), s)
+                                          : launch<128>(stats_kernel<128>, p, tiles_of(p.cols, p.N, 128), s);
+}
+int32_t logits_dz(const Logits& p, hipStream_t s) { return launch<256>(dz_kernel, p, tiles_of(p.cols, p.N, 256), s); }
 int32_t gradient(const Gradient& q, hipStream_t s) {
   Gradient p = q;
   p.vec = !p.by_a && p.ld % 4 == 0 && p.rows_a % 4 == 0 && p.part_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-  return launch(gradient_kernel, p, ceil_div64(p.rows_a, kPanel) * ceil_div64(p.rows_b, kPanel) * p.parts, s);
+  return product_tile(p.rows_a, p.rows_b) == 256 ? launch<256>(gradient_kernel<256>, p, tiles_of(p.rows_a, p.rows_b, 256) * p.parts, s)
+                                                 : launch<128>(gradient_kernel<128>, p, tiles_of(p.rows_a, p.rows_b, 128) * p.parts, s);
 }
 
 }  // namespace lce

@@ -54,6 +54,7 @@ struct Gradient {
   const float *g, *count;
 };
 int32_t gradient(const Gradient& a, hipStream_t s);
+int product_tile(int64_t a, int64_t b);  // edge of the tiles that a product of a x b rows is cut into: 256 or 128
 
 // The largest finite magnitude of every row of an operand (as pack takes it).
 int32_t row_amax(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, float* amax, hipStream_t s);
@@ -93,7 +94,7 @@ struct Outer {
   int64_t dz_ld, N, D, cols;
   float* out;
   int64_t ld;
-  int groups;  // of 128 of x's columns per work-group (set by direct_dw)
+  int groups;  // of 128 (pairs: 256) of x's columns per work-group (set by direct_dw)
   const float *g, *count;
 };
 int32_t direct_dw(const Outer& p, bool by_d, hipStream_t s);

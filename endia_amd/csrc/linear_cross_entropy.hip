@@ -231,7 +231,7 @@ int64_t panel_columns(int64_t N, int64_t D, int64_t V, bool backward) {
 
 int32_t many_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,
                       float* loss, float* lse, hipStream_t s) {
-  const int64_t piece = panel_columns(N, D, V, false), tiles = ceil_div64(piece, lce::kPanel);
+  const int64_t piece = panel_columns(N, D, V, false), tiles = ceil_div64(piece, 128);
   Scratch w;
   const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N),
                 st = w.want(8 * tiles * N), run = w.want(12 * N);
@@ -246,7 +246,7 @@ int32_t many_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
     a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
     a.stats = w.f(st); a.zt = zt;
     if ((rc = lce::logits_stats(a, s))) return rc;
-    if ((rc = join_stats(w.f(st), ceil_div64(cols, lce::kPanel), N, m, l, v0 == 0, s))) return rc;
+    if ((rc = join_stats(w.f(st), ceil_div64(cols, lce::product_tile(cols, N)), N, m, l, v0 == 0, s))) return rc;
   }
   hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(TPB), 0, s, N, V, target, m, l, zt, lse, loss);
   ENDIA_LAUNCH_CHECK();
@@ -256,8 +256,12 @@ int32_t many_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
 int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,
                       const float* lse, const float* g, float* dx, float* dW, hipStream_t s) {
   const int64_t piece = panel_columns(N, D, V, true), rows = ceil_div64(N, lce::kPanel) * lce::kPanel, ptiles = ceil_div64(piece, lce::kPanel);
-  const int64_t d_tiles = ceil_div64(D, lce::kPanel), cus = ctx().cu_count;
-  const int parts = cut(rows / lce::kPanel * d_tiles, cus, ptiles, 16), w_parts = cut(ptiles * d_tiles, cus, rows / lce::kPanel, 16);
+  // a gradient of few tiles and a long k: k is cut until the chip is full
+  auto parts_of = [&](int64_t a, int64_t b, int64_t panels) {
+    const int64_t T = lce::product_tile(a, b);
+    return cut(ceil_div64(a, T) * ceil_div64(b, T), T == 256 ? ctx().cu_count : 2 * ctx().cu_count, panels, 16);
+  };
+  const int parts = parts_of(D, N, ptiles), w_parts = parts_of(D, piece, rows / lce::kPanel);
   Scratch w;
   const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N),
                 xt = w.want(dW ? lce::panel_bytes(D, N) : 0), xta = w.want(4 * D), wt = w.want(dx ? lce::panel_bytes(D, piece) : 0), wta = w.want(4 * D),
