@@ -48,7 +48,7 @@ struct Args {
   float* part;       // partial results of a split walk
   float* part_ml;    // forward: running maximum (base 2) and sum of each partial result
   float* part_table; // per work-group sums of ds by position difference
-  float* part_rows;  // per row and part: sum of ds, sums of p in the two last buckets
+  float* part_rows;  // per row and part: sums of ds and of p in the two last buckets, of p and of ds over all (8 floats)
   int splits;
   int stages;  // tiles that dq_kernel's LDS holds
   Buckets bk;

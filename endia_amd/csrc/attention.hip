@@ -180,7 +180,7 @@ int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* 
   const int64_t part_q = aq.splits > 1 ? 4 * aq.splits * a.B * a.Q * a.H * a.D : 0, part_k = ak.splits > 1 ? 8 * ak.splits * a.B * a.K * a.Hk * a.D : 0;
   const int64_t part = w.want(part_q > part_k ? part_q : part_k);  // (one after the other on the stream)
   const int64_t span = 2 * a.bk.near + 1, table_part = w.want(dtable ? table_groups(aq) * span * 4 : 0), diff = w.want(dtable ? 8 * a.H * span : 0),
-                table_rows = w.want(dtable && aq.splits > 1 ? 16 * a.B * a.H * a.Q * aq.splits : 0);
+                table_rows = w.want(dtable && aq.splits > 1 ? 32 * a.B * a.H * a.Q * aq.splits : 0);
   if ((rc = w.get())) return rc;
   for (Args* x : {&a, &aq, &ak}) {
     x->k_rows = w.at<char>(kr); x->k_cols = w.at<char>(kc); x->v_rows = w.at<char>(vr); x->q_rows = w.at<char>(qr);

@@ -16,7 +16,6 @@ namespace {
 
 using namespace pairs;
 constexpr int TPB = 256;
-static_assert(2 * kMaxSide <= TPB, "table_grad_kernel gives every bucket a thread");
 constexpr float kMost = 32768.f;  // a scaled p or ds stays below this
 
 // Brings the running shift F of the lane's accumulator column (2^F times the sums; both halves of the wave agree on it) and the
@@ -74,6 +73,10 @@ __device__ __forceinline__ void store_row(float* out, const floatx16 (&acc)[DP /
     }
 }
 
+__device__ __forceinline__ float far_part(float ds, float p, float p_all, float row_sum) {
+  return p_all > 0.f ? (ds - p * (row_sum / p_all)) / p_all : ds;
+}
+
 template <int DP, bool BIAS>
 __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const int* __restrict__ k_shift, const int* __restrict__ v_shift,
                                                                    const float* __restrict__ meta) {
@@ -98,7 +101,15 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
   const int64_t iv = min(i, a.Q - 1);
   const int qshift = load_fragments<DP>(a.q + b * a.qs[0] + iv * a.qs[1] + h * a.qs[2], in, D, a.vec, half, qh, ql);
   const int gshift = load_fragments<DP>(a.go + ((b * a.Q + iv) * a.H + h) * D, in, D, a.vec, half, gh, gl);
-  const float cq = a.scale * kLog2e * pow2i(-qshift), cg = pow2i(-gshift);
+  // The matrix instruction's sums are a little low on average (3e-8 of |do| |v| here, far below one rounding), which shows where
+  // ds is added up over a million pairs: every other query's dp is formed with its sign turned, so that it cancels over the rows.
+  const float turn = col & 1 ? -1.f : 1.f;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    gh[s] *= (_Float16)turn;
+    gl[s] *= (_Float16)turn;
+  }
+  const float cq = a.scale * kLog2e * pow2i(-qshift), cg = turn * pow2i(-gshift);
   const int64_t qtiles = (a.Q + kTile - 1) / kTile;
   const int64_t mt = ((b * a.H + h) * qtiles + min(q0 / 32, qtiles - 1)) * 64;
   const float lse = in ? meta[mt + col] : INFINITY, delta = in ? meta[mt + 32 + col] : 0.f;
@@ -108,9 +119,10 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
       for (int j = tid; j < 4 * span; j += TPB) bins[j] = 0.f;
   }
   float* my_bins = bins + wave * span;
-  // The sum of a row's ds is zero, and a bucket far away holds most of it: what delta is off by (it comes from the rounded o)
-  // would add up there over all keys. So the row's own sum is taken too, and the far buckets give it back by their part of p.
-  float far_low = 0.f, far_high = 0.f, p_low = 0.f, p_high = 0.f, row_sum = 0.f;
+  // The sum of a row's p is 1, that of its ds 0, and a bucket far away holds most of both: what lse and delta are off by (they come
+  // from rounded results) would add up there over all keys. So the row's own sums are taken too, and the far buckets' are set right
+  // by them: ds_far := (ds_far - p_far sum(ds) / sum(p)) / sum(p).
+  float far_low = 0.f, far_high = 0.f, p_low = 0.f, p_high = 0.f, p_all = 0.f, row_sum = 0.f;
 
   const int n = key_count(a, b);
   const int64_t place = i + a.off;
@@ -194,12 +206,15 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[v] = in && key0 + 8 * (v >> 2) + (v & 3) < limit ? x[v] : 0.f;
       }
-      if (sum_table && far) {
+      if (sum_table) {
         float sum = 0.f;
 #pragma unroll
         for (int v = 0; v < 16; ++v) sum += x[v];
-        if (hi <= -near) p_low += sum;
-        else p_high += sum;
+        p_all += sum;
+        if (far) {
+          if (hi <= -near) p_low += sum;
+          else p_high += sum;
+        }
       }
 #pragma unroll
       for (int v = 0; v < 16; ++v) x[v] *= dp[v] * cd - delta;
@@ -247,18 +262,18 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
   }
   if (sum_table) {
     // (both halves of the wave hold parts of a row)
-    row_sum += __shfl_xor(row_sum, 32, 64);
+    float* sums[] = {&far_low, &far_high, &p_low, &p_high, &p_all, &row_sum};
+#pragma unroll
+    for (float* x : sums) *x += __shfl_xor(*x, 32, 64);
     if (a.splits == 1) {
-      far_low -= row_sum * p_low;
-      far_high -= row_sum * p_high;
-    } else {
-      p_low += __shfl_xor(p_low, 32, 64);
-      p_high += __shfl_xor(p_high, 32, 64);
-      if (in && half == 0) {
-        float* to = a.part_rows + (((b * a.H + h) * a.Q + i) * a.splits + split) * 4;
-        *reinterpret_cast<float4*>(to) = make_float4(row_sum, p_low, p_high, 0.f);
-      }
+      far_low = far_part(far_low, p_low, p_all, row_sum);
+      far_high = far_part(far_high, p_high, p_all, row_sum);
+    } else if (in && half == 0) {  // a row that is cut: table_grad_kernel adds its parts up first
+      float4* to = reinterpret_cast<float4*>(a.part_rows + (((b * a.H + h) * a.Q + i) * a.splits + split) * 8);
+      to[0] = make_float4(far_low, far_high, p_low, p_high);
+      to[1] = make_float4(p_all, row_sum, 0.f, 0.f);
     }
+    if (a.splits > 1 || half) far_low = far_high = 0.f;
     // the wave's far sums join its bins at the ends, then the waves' bins are added in order
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
@@ -458,7 +473,7 @@ __global__ __launch_bounds__(TPB) void table_diff_kernel(Args a, int64_t per_hea
   if (run == 0 && d < span) diff[h * span + d] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
-// dtable[bucket, h] from the sums by difference; what the far buckets give back of their rows' sums where a row was cut in parts.
+// dtable[bucket, h] from the sums by difference, and from the rows' far sums where rows were cut in parts.
 __global__ __launch_bounds__(TPB) void table_grad_kernel(Args a, const double* __restrict__ diff, float* __restrict__ dtable) {
   __shared__ double red[2][TPB];
   const int span = 2 * a.bk.near + 1, tid = threadIdx.x, buckets = a.bk.both ? 2 * a.bk.side : a.bk.side;
@@ -466,16 +481,14 @@ __global__ __launch_bounds__(TPB) void table_grad_kernel(Args a, const double* _
   double low = 0.0, high = 0.0;
   if (a.splits > 1)
     for (int64_t r = tid; r < a.B * a.Q; r += TPB) {
-      const float* from = a.part_rows + ((r / a.Q * a.H + h) * a.Q + r % a.Q) * a.splits * 4;
-      float sum = 0.f, pl = 0.f, ph = 0.f;
+      const float* from = a.part_rows + ((r / a.Q * a.H + h) * a.Q + r % a.Q) * a.splits * 8;
+      float sum[6] = {};
       for (int s = 0; s < a.splits; ++s) {
-        const float4 f = *reinterpret_cast<const float4*>(from + s * 4);
-        sum += f.x;
-        pl += f.y;
-        ph += f.z;
+        const float4 f = *reinterpret_cast<const float4*>(from + s * 8), g = *reinterpret_cast<const float4*>(from + s * 8 + 4);
+        sum[0] += f.x; sum[1] += f.y; sum[2] += f.z; sum[3] += f.w; sum[4] += g.x; sum[5] += g.y;
       }
-      low += (double)(sum * pl);
-      high += (double)(sum * ph);
+      low += (double)far_part(sum[0], sum[2], sum[4], sum[5]);
+      high += (double)far_part(sum[1], sum[3], sum[4], sum[5]);
     }
   red[0][tid] = low;
   red[1][tid] = high;
@@ -487,25 +500,17 @@ __global__ __launch_bounds__(TPB) void table_grad_kernel(Args a, const double* _
     }
     __syncthreads();
   }
-  // (the differences of a bucket lie side by side; 256 at a time wait in LDS)
-  __shared__ double part[TPB];
-  __shared__ int of[TPB];
-  double sum = 0.0;
-  const int bucket = tid;
-  for (int d0 = 0; d0 < span; d0 += TPB) {
-    __syncthreads();
-    if (d0 + tid < span) {
-      part[tid] = diff[h * span + d0 + tid];
-      of[tid] = bucket_of(a.bk, d0 + tid - a.bk.near);
-    }
-    __syncthreads();
-    if (bucket < buckets)
-      for (int d = 0; d < min(TPB, span - d0); ++d) sum += of[d] == bucket ? part[d] : 0.0;
-  }
-  if (bucket < buckets) {
-    if (bucket == bucket_of(a.bk, -a.bk.near)) sum -= red[0][0];
-    if (bucket == bucket_of(a.bk, a.bk.near)) sum -= red[1][0];
-    dtable[bucket * a.H + h] = (float)sum;
+  // A bucket's differences lie side by side: a wave adds up one bucket after another.
+  const int lane = tid & 63;
+  for (int bucket = tid >> 6; bucket < buckets; bucket += TPB / 64) {
+    double sum = 0.0;
+    for (int d = lane; d < span; d += 64)
+      if (bucket_of(a.bk, d - a.bk.near) == bucket) sum += diff[h * span + d];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (bucket == bucket_of(a.bk, -a.bk.near)) sum += red[0][0];
+    if (bucket == bucket_of(a.bk, a.bk.near)) sum += red[1][0];
+    if (lane == 0) dtable[bucket * a.H + h] = (float)sum;
   }
 }
 
