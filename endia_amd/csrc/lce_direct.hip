@@ -113,7 +113,8 @@ template <bool KCONTIG, typename Op>
 __global__ __launch_bounds__(TPB) void planes_kernel(const float* __restrict__ x, int64_t ld, int64_t rows, int64_t k, const float* __restrict__ left_out,
                                                      const float* __restrict__ amax, char* __restrict__ planes) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int64_t steps = (k + 15) / 16, step = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), block = blockIdx.y, r = block * 32 + (lane & 31);
+  const int64_t steps = (k + 15) / 16, step_groups = (steps + 3) / 4;
+  const int64_t step = blockIdx.x % step_groups * 4 + (threadIdx.x >> 6), block = blockIdx.x / step_groups, r = block * 32 + (lane & 31);
   if (step >= steps) return;
   float v[8];
   load_step<KCONTIG>(x, ld, r, rows, step * 16, k, half, v);
@@ -496,7 +497,7 @@ int32_t stream(const Direct& p, bool kcontig, hipStream_t s) {
 }  // namespace
 
 int32_t planes(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, const float* amax, char* to, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div64(ceil_div64(k, 16), 4), (unsigned)ceil_div64(rows, 32));
+  const dim3 grid((unsigned)(ceil_div64(ceil_div64(k, 16), 4) * ceil_div64(rows, 32)));
   if (transposed && amax) hipLaunchKernelGGL((planes_kernel<false, Pair>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);
   else if (transposed) hipLaunchKernelGGL((planes_kernel<false, Triple>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);
   else if (amax) hipLaunchKernelGGL((planes_kernel<true, Pair>), grid, dim3(TPB), 0, s, x, ld, rows, k, left_out, amax, to);

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(TPB) void pack_cols_kernel(const float* __restrict_
                                                         char* __restrict__ panels, const float* __restrict__ amax) {
   __shared__ float t[kBlock][129];
   const int tid = threadIdx.x;
-  const int64_t r0 = (int64_t)blockIdx.x * 128, kb = blockIdx.y, kblocks = (k + kBlock - 1) / kBlock;
+  const int64_t row_groups = (rows + 127) / 128, r0 = blockIdx.x % row_groups * 128, kb = blockIdx.x / row_groups, kblocks = (k + kBlock - 1) / kBlock;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int kk = i * 2 + (tid >> 7), rr = tid & 127;
@@ -134,7 +134,7 @@ int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t 
   }
   int32_t rc = known ? ENDIA_HIP_OK : row_amax(x, ld, true, rows, k, left_out, amax, s);
   if (rc) return rc;
-  hipLaunchKernelGGL(pack_cols_kernel, dim3((unsigned)ceil_div64(rows, 128), (unsigned)ceil_div64(k, kBlock)), dim3(TPB), 0, s, x, ld, rows, k, left_out,
+  hipLaunchKernelGGL(pack_cols_kernel, dim3((unsigned)(ceil_div64(rows, 128) * ceil_div64(k, kBlock))), dim3(TPB), 0, s, x, ld, rows, k, left_out,
                      panels, amax);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;

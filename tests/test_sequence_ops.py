@@ -622,6 +622,96 @@ def test_linear_cross_entropy_python_refusals():
         nd.linear_cross_entropy(x, w, t).backward(create_graph=True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape, tied", [((129, 300, 1001), False), ((200, 513, 700), True), ((511, 260, 1500), False), ((390, 33, 5001), True),
+                                         ((33, 1030, 640), False), ((20, 70, 40000), True), ((1100, 300, 3001), False), ((1030, 520, 700), True),
+                                         ((2600, 20, 900), False), ((600, 1400, 300), True)])
+def test_linear_cross_entropy_between_the_kernels(shape, tied):
+    """Either side of the changes of kernel by rows, classes and width: several column tiles, cut reductions, ragged everything."""
+    check_loss(*shape, tied=tied)
+
+
+@pytest.mark.gpu
+def test_linear_cross_entropy_selected_gradients():
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    for N in (9, 100, 600):
+        x, w = rng.standard_normal((N, 40)).astype(np.float32), rng.standard_normal((40, 300)).astype(np.float32)
+        t = rng.integers(0, 300, N).astype(np.float32)
+        want = loss_reference(x, w, t)
+        for i, n in enumerate(("dx", "dw")):
+            arrays = [nd.array(a, requires_grad=j == i) for j, a in enumerate((x, w))]
+            loss = nd.linear_cross_entropy(*arrays, nd.array(t))
+            within(nd.grad(outs=[loss], inputs=[arrays[i]])[0].to_numpy(), want[n], n)
+
+
+@pytest.mark.gpu
+def test_linear_cross_entropy_of_one_vector_and_of_a_shared_array():
+    """x without a rows axis; the rows and the classes' weights one and the same array."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal(24).astype(np.float32), rng.standard_normal((24, 50)).astype(np.float32)
+    want = loss_reference(x[None], w, np.array([7.0]))
+    xa = nd.array(x, requires_grad=True)
+    loss = nd.linear_cross_entropy(xa, nd.array(w), nd.array(np.array([7.0], np.float32)))
+    within(loss.to_numpy(), want["loss"])
+    within(nd.grad(outs=[loss], inputs=[xa])[0].to_numpy(), want["dx"])
+    e = rng.standard_normal((70, 24)).astype(np.float32)
+    t = np.arange(70, dtype=np.float32)[::-1].copy()
+    want = loss_reference(e, e.T, t)
+    ea = nd.array(e, requires_grad=True)
+    loss = nd.linear_cross_entropy(ea, ea.T(), nd.array(t))
+    got = nd.grad(outs=[loss], inputs=[ea])[0].to_numpy()
+    both = want["dx"][0] + want["dw"][0].T, want["dx"][1] + want["dw"][1].T + 4 * U * (np.abs(want["dx"][0]) + np.abs(want["dw"][0].T))
+    within(got, both, "dx + dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 65])
+def test_attention_of_one_array_to_itself(T):
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    x, go = (rng.standard_normal((2, T, 3, 32)).astype(np.float32) for _ in range(2))
+    xa = nd.array(x, requires_grad=True)
+    o = nd.attention(xa, xa, xa, causal=True)
+    want = attention_reference(x, x, x, go, causal=True)
+    within(o.to_numpy(), want["o"], "o")
+    got = nd.grad(outs=[o], inputs=[xa], grad_outs=[nd.array(go)])[0].to_numpy()
+    value = sum(want[n][0] for n in ("dq", "dk", "dv"))
+    within(got, (value, sum(want[n][1] + 4 * U * np.abs(want[n][0]) for n in ("dq", "dk", "dv"))), "dq + dk + dv")
+
+
+@pytest.mark.gpu
+def test_two_captured_steps_share_nothing():
+    """Two captured steps of different sizes, replayed in turn, and eager calls between them."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    steps = []
+    for N, V, T in ((40, 300, 20), (700, 900, 150)):
+        x = nd.array(rng.standard_normal((N, 48)).astype(np.float32), requires_grad=True)
+        w = nd.array(rng.standard_normal((48, V)).astype(np.float32), requires_grad=True)
+        t = nd.array(rng.integers(0, V, N).astype(np.float32))
+        q = nd.array(rng.standard_normal((1, T, 4, 64)).astype(np.float32), requires_grad=True)
+        table = nd.array(rng.standard_normal((16, 4)).astype(np.float32), requires_grad=True)
+        go = nd.array(rng.standard_normal((1, T, 4, 64)).astype(np.float32))
+
+        def step(x=x, w=w, t=t, q=q, table=table, go=go):
+            loss = nd.linear_cross_entropy(x, w, t)
+            o = nd.relative_attention(q, q, q, table, max_distance=30)
+            return [loss, o] + nd.grad(outs=[loss], inputs=[x, w]) + nd.grad(outs=[o], inputs=[q, table], grad_outs=[go])
+
+        eager = [a.to_numpy() for a in step()]
+        steps.append((nd.capture(step), eager))
+    for turn in (0, 1, 1, 0, 1, 0, 0, 1):
+        captured, eager = steps[turn]
+        captured.replay()
+        check_attention(1, 40, 60, 2, 2, 64)
+        for a, b in zip(captured.outputs, eager):
+            assert np.array_equal(a.to_numpy(), b), turn
+    for captured, _ in steps:
+        captured.close()
+
+
 # ---- together -------------------------------------------------------------------------------------------------
 def _little_model(nd, rng, B, T, S, H, D, V):
     """One decoder layer: causal self attention with position buckets, cross attention to encoder states, tied loss."""
