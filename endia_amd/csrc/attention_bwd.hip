@@ -85,13 +85,13 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
   const int near = a.bk.near, span = 2 * near + 1;
   float* bias_lds = reinterpret_cast<float*>(smem + a.stages * STAGE);
   float* bins = bias_lds + span;  // one set per wave: sums of ds by position difference
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int64_t qgroups = (a.Q + 127) / 128;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const uint32_t split = id % (uint32_t)a.splits;
   id /= (uint32_t)a.splits;
   const uint32_t hb = id / (uint32_t)qgroups;
-  const int64_t qt = id % (uint32_t)qgroups, h = hb % (uint32_t)a.H, b = hb / (uint32_t)a.H, kh = (uint32_t)h / (uint32_t)a.G;
+  const int64_t qt = a.causal ? qgroups - 1 - id % (uint32_t)qgroups : id % (uint32_t)qgroups, h = hb % (uint32_t)a.H, b = hb / (uint32_t)a.H, kh = (uint32_t)h / (uint32_t)a.G;
   const int D = (int)a.D;
   const int64_t q0 = qt * 128 + wave * 32, i = q0 + col;
   const bool in = i < a.Q;
@@ -296,8 +296,9 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
   constexpr int STAGE = DP * 512 + 256;  // row and column images of q and do; lse and delta
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* bias_lds = reinterpret_cast<float*>(smem + 2 * STAGE);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int near = a.bk.near, span = 2 * near + 1;
+  const int tid = threadIdx.x, lane = tid & 63, wave = BIAS ? __builtin_amdgcn_readfirstlane(tid >> 6) : tid >> 6, col = lane & 31, half = lane >> 5;
+  const int near = a.bk.near;  // (with a table the wave's number is made scalar: its addresses then need no vector registers, 1.03 ms
+                               // against 1.35 at 5001 causal queries; without one the scalar registers run out instead, 4.0 against 3.7)
   const int64_t kgroups = (a.K + 127) / 128;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const uint32_t split = id % (uint32_t)a.splits;
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
           dp = mfma_pairs(ah, al, vfh[2 * kb + st], vfl[2 * kb + st], dp);
         }
       const float c = ck * pow2i(-qs), cd = cv * pow2i(-gs);
-      float p[16], x[16];
+      float p[16];
 #pragma unroll
       for (int v = 0; v < 16; ++v) p[v] = s[v] * c;
       if (BIAS) {
@@ -393,24 +394,17 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float4 e = *reinterpret_cast<const float4*>(row_lse + 8 * g + 4 * half);
-        const float4 dl = *reinterpret_cast<const float4*>(row_lse + 32 + 8 * g + 4 * half);
         p[4 * g] = exp2_fast(p[4 * g] - e.x);
         p[4 * g + 1] = exp2_fast(p[4 * g + 1] - e.y);
         p[4 * g + 2] = exp2_fast(p[4 * g + 2] - e.z);
         p[4 * g + 3] = exp2_fast(p[4 * g + 3] - e.w);
-        x[4 * g] = p[4 * g] * (dp[4 * g] * cd - dl.x);
-        x[4 * g + 1] = p[4 * g + 1] * (dp[4 * g + 1] * cd - dl.y);
-        x[4 * g + 2] = p[4 * g + 2] * (dp[4 * g + 2] * cd - dl.z);
-        x[4 * g + 3] = p[4 * g + 3] * (dp[4 * g + 3] * cd - dl.w);
       }
-      if (k0 + 31 >= n || q0 + 31 >= a.Q || (a.causal && p0 < k0 + 31)) {
+      const bool mask = k0 + 31 >= n || q0 + 31 >= a.Q || (a.causal && p0 < k0 + 31);
+      // the first and the last of the tile's queries that see the lane's key, counted from the lane's first one
+      const int from = a.causal ? (int)max(min(j - p0, (int64_t)32), (int64_t)0) - 4 * half : -4, to = in ? (int)min(a.Q - q0, (int64_t)32) - 4 * half : -4;
+      if (mask) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int64_t q = q0 + 8 * (v >> 2) + 4 * half + (v & 3);
-          const bool left = in && q < a.Q && (!a.causal || q + a.off >= j);
-          p[v] = left ? p[v] : 0.f;
-          x[v] = left ? x[v] : 0.f;
-        }
+        for (int v = 0; v < 16; ++v) p[v] = 8 * (v >> 2) + (v & 3) >= from && 8 * (v >> 2) + (v & 3) < to ? p[v] : 0.f;
       }
       half8 xh[2], xl[2];
       as_operand(p, fit<DP / 32>(p, gs, FV, dv), xh, xl);
@@ -422,7 +416,19 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
           read_line(gcol, d * 32 + col, st, half, ah, al);
           dv[d] = mfma_pairs(ah, al, xh[st], xl[st], dv[d]);
         }
-      as_operand(x, fit<DP / 32>(x, qs, FK, dk), xh, xl);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 dl = *reinterpret_cast<const float4*>(row_lse + 32 + 8 * g + 4 * half);
+        p[4 * g] *= dp[4 * g] * cd - dl.x;
+        p[4 * g + 1] *= dp[4 * g + 1] * cd - dl.y;
+        p[4 * g + 2] *= dp[4 * g + 2] * cd - dl.z;
+        p[4 * g + 3] *= dp[4 * g + 3] * cd - dl.w;
+      }
+      if (mask) {  // (p = 0 leaves 0 only where dp is finite)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) p[v] = 8 * (v >> 2) + (v & 3) >= from && 8 * (v >> 2) + (v & 3) < to ? p[v] : 0.f;
+      }
+      as_operand(p, fit<DP / 32>(p, qs, FK, dk), xh, xl);
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -501,11 +507,14 @@ __global__ __launch_bounds__(TPB) void table_grad_kernel(Args a, const double* _
     __syncthreads();
   }
   // A bucket's differences lie side by side: a wave adds up one bucket after another.
-  const int lane = tid & 63;
-  for (int bucket = tid >> 6; bucket < buckets; bucket += TPB / 64) {
+  const int lane = tid & 63, near = a.bk.near;
+  for (int bucket = __builtin_amdgcn_readfirstlane(tid >> 6); bucket < buckets; bucket += TPB / 64) {
+    const bool later = bucket >= a.bk.side;  // two sides: keys behind the query
+    const int i = later ? bucket - a.bk.side : bucket;
+    const int n0 = a.bk.start[i], n1 = i + 1 < a.bk.side ? a.bk.start[i + 1] - 1 : near;
+    const int first = later ? near + max(n0, 1) : near - n1, last = later ? near + n1 : (!a.bk.both && i == 0 ? 2 * near : near - n0);
     double sum = 0.0;
-    for (int d = lane; d < span; d += 64)
-      if (bucket_of(a.bk, d - a.bk.near) == bucket) sum += diff[h * span + d];
+    for (int d = first + lane; d <= last; d += 64) sum += diff[h * span + d];
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if (bucket == bucket_of(a.bk, -a.bk.near)) sum += red[0][0];

@@ -25,13 +25,14 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __re
   constexpr int STAGE = DP * 256;  // row image of k, column image of v
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* bias_lds = reinterpret_cast<float*>(smem + 2 * STAGE);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int64_t qtiles = (a.Q + 127) / 128;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const uint32_t split = id % (uint32_t)a.splits;
   id /= (uint32_t)a.splits;
   const uint32_t hb = id / (uint32_t)qtiles;
-  const int64_t qt = id % (uint32_t)qtiles, h = hb % (uint32_t)a.H, b = hb / (uint32_t)a.H, kh = (uint32_t)h / (uint32_t)a.G;
+  // (causal: the last queries see the most keys and go first)
+  const int64_t qt = a.causal ? qtiles - 1 - id % (uint32_t)qtiles : id % (uint32_t)qtiles, h = hb % (uint32_t)a.H, b = hb / (uint32_t)a.H, kh = (uint32_t)h / (uint32_t)a.G;
   const int D = (int)a.D;
   const int64_t i = qt * 128 + wave * 32 + col;
   const bool in = i < a.Q;

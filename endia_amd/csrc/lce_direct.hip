@@ -212,7 +212,7 @@ template <bool KCONTIG, int MODE>
 __global__ __launch_bounds__(TPB, 2) void stream_few_kernel(Direct p) {
   constexpr int CS = 4;
   __shared__ float red[4][16][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * 32;
   const int part = blockIdx.z;
   const int steps = (int)((p.k + 15) / 16), chunks = (steps + CS - 1) / CS, per = (chunks + p.parts - 1) / p.parts;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   constexpr int CS = NB > 2 ? 2 : 4;  // steps per chunk
   constexpr int STAGE = CS * NB * step_bytes<Op>(), P = Op::PARTS;
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   // Work-groups are dealt round-robin to the 8 XCDs: those that read the same 128 rows for different columns follow each other on
   // one XCD, so that the rows come from memory once and then from its L2.
   const int ntiles = (int)((p.N + NB * 32 - 1) / (NB * 32)), turn = blockIdx.x >> 3;
@@ -374,7 +374,7 @@ template <bool BY_D, typename Op>
 __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
   constexpr int P = Op::PARTS, DB = P == 2 ? 8 : 4, CS = 2, STAGE = DB * CS * step_bytes<Op>();
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int64_t v0 = (int64_t)blockIdx.x * 128 + wave * 32, v = v0 + col;
   const int steps = (int)((p.N + 15) / 16), chunks = (steps + CS - 1) / CS, blocks = (int)((p.D + 31) / 32);
   const int groups = (blocks + DB - 1) / DB, g0 = blockIdx.y * p.groups, g1 = min(g0 + p.groups, groups);
