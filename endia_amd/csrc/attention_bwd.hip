@@ -297,8 +297,8 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* bias_lds = reinterpret_cast<float*>(smem + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = BIAS ? __builtin_amdgcn_readfirstlane(tid >> 6) : tid >> 6, col = lane & 31, half = lane >> 5;
-  const int near = a.bk.near;  // (with a table the wave's number is made scalar: its addresses then need no vector registers, 1.03 ms
-                               // against 1.35 at 5001 causal queries; without one the scalar registers run out instead, 4.0 against 3.7)
+  const int near = a.bk.near;  // (with a table the wave's number is made scalar, so that addresses take no vector registers: with the
+                               // order of ds below 1.03 ms against 1.35 at 5001 causal queries and 16 heads of 128)
   const int64_t kgroups = (a.K + 127) / 128;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const uint32_t split = id % (uint32_t)a.splits;
@@ -406,6 +406,24 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
 #pragma unroll
         for (int v = 0; v < 16; ++v) p[v] = 8 * (v >> 2) + (v & 3) >= from && 8 * (v >> 2) + (v & 3) < to ? p[v] : 0.f;
       }
+      // ds, before dv's products (more for the vector ALU to do beside them: 3.7 ms against 4.0 at 4096 x 16384) or, where the table
+      // leaves no registers for both p and ds, behind them
+      float x[16];
+      auto form_ds = [&]() {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 dl = *reinterpret_cast<const float4*>(row_lse + 32 + 8 * g + 4 * half);
+          x[4 * g] = p[4 * g] * (dp[4 * g] * cd - dl.x);
+          x[4 * g + 1] = p[4 * g + 1] * (dp[4 * g + 1] * cd - dl.y);
+          x[4 * g + 2] = p[4 * g + 2] * (dp[4 * g + 2] * cd - dl.z);
+          x[4 * g + 3] = p[4 * g + 3] * (dp[4 * g + 3] * cd - dl.w);
+        }
+        if (mask) {  // (p = 0 leaves 0 only where dp is finite)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[v] = 8 * (v >> 2) + (v & 3) >= from && 8 * (v >> 2) + (v & 3) < to ? x[v] : 0.f;
+        }
+      };
+      if (!BIAS) form_ds();
       half8 xh[2], xl[2];
       as_operand(p, fit<DP / 32>(p, gs, FV, dv), xh, xl);
 #pragma unroll
@@ -416,19 +434,8 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
           read_line(gcol, d * 32 + col, st, half, ah, al);
           dv[d] = mfma_pairs(ah, al, xh[st], xl[st], dv[d]);
         }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float4 dl = *reinterpret_cast<const float4*>(row_lse + 32 + 8 * g + 4 * half);
-        p[4 * g] *= dp[4 * g] * cd - dl.x;
-        p[4 * g + 1] *= dp[4 * g + 1] * cd - dl.y;
-        p[4 * g + 2] *= dp[4 * g + 2] * cd - dl.z;
-        p[4 * g + 3] *= dp[4 * g + 3] * cd - dl.w;
-      }
-      if (mask) {  // (p = 0 leaves 0 only where dp is finite)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) p[v] = 8 * (v >> 2) + (v & 3) >= from && 8 * (v >> 2) + (v & 3) < to ? p[v] : 0.f;
-      }
-      as_operand(p, fit<DP / 32>(p, qs, FK, dk), xh, xl);
+      if (BIAS) form_ds();
+      as_operand(x, fit<DP / 32>(x, qs, FK, dk), xh, xl);
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll

@@ -270,11 +270,12 @@ __global__ __launch_bounds__(TPB, 2) void stream_kernel(Direct p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   // Work-groups are dealt round-robin to the 8 XCDs: those that read the same 128 rows for different columns follow each other on
   // one XCD, so that the rows come from memory once and then from its L2.
-  const int ntiles = (int)((p.N + NB * 32 - 1) / (NB * 32)), turn = blockIdx.x >> 3;
-  const int64_t group = (int64_t)(turn / ntiles) * 8 + (blockIdx.x & 7);
+  const uint32_t ntiles = (uint32_t)((p.N + NB * 32 - 1) / (NB * 32)), turn = blockIdx.x >> 3;
+  const uint32_t unit = turn / ntiles * 8 + (blockIdx.x & 7);  // of rows and part
+  const int64_t group = unit / (uint32_t)p.parts;
   if (group * 128 >= p.rows) return;
   const int64_t r0 = group * 128 + wave * 32;
-  const int n0 = turn % ntiles * NB * 32, part = blockIdx.y;
+  const int n0 = (int)(turn % ntiles) * NB * 32, part = (int)(unit % (uint32_t)p.parts);
   const int steps = (int)((p.k + 15) / 16), chunks = (steps + CS - 1) / CS, per = (chunks + p.parts - 1) / p.parts;
   const int c0 = min(part * per, chunks), c1 = min(c0 + per, chunks);
   const int blocks = (int)((p.N + 31) / 32), first_block = n0 / 32;
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
 
 template <int NB, typename Op, int MODE>
 int32_t stream_tiles(const Direct& p, bool kcontig, hipStream_t s) {
-  const dim3 grid((unsigned)(ceil_div64(ceil_div64(p.rows, 128), 8) * 8 * ceil_div64(p.N, NB * 32)), (unsigned)p.parts);
+  const dim3 grid((unsigned)(ceil_div64(ceil_div64(p.rows, 128) * p.parts, 8) * 8 * ceil_div64(p.N, NB * 32)));
   if (kcontig) hipLaunchKernelGGL((stream_kernel<NB, Op, true, MODE>), grid, dim3(TPB), 0, s, p);
   else hipLaunchKernelGGL((stream_kernel<NB, Op, false, MODE>), grid, dim3(TPB), 0, s, p);
   ENDIA_LAUNCH_CHECK();

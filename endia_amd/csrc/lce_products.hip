@@ -27,7 +27,7 @@ struct Tile {
   int lane, wave, col, half, wa, wb;  // the wave's place along a and b
   __device__ __forceinline__ Tile() {
     lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (known to be uniform: addresses that depend on it stay scalar)
+    wave = threadIdx.x >> 6;
     col = lane & 31;
     half = lane >> 5;
     wa = wave / WB;
