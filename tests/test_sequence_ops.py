@@ -682,6 +682,25 @@ def test_attention_of_one_array_to_itself(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [4, 50])
+def test_attention_under_a_mean_and_behind_a_product(T):
+    """The cotangent of a mean is one number spread out; the output also meets an elementwise product first."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    q, k, v, w = (rng.standard_normal((2, n, 2, 32)).astype(np.float32) for n in (T, 40, 40, T))
+    n = q.size
+    for weights in (None, w):
+        arrays = [nd.array(a, requires_grad=True) for a in (q, k, v)]
+        o = nd.attention(*arrays)
+        nd.mean(o if weights is None else o * nd.array(weights)).backward()
+        go = (np.ones_like(q) if weights is None else weights) / np.float32(n)
+        want = attention_reference(q, k, v, go)
+        for a, name in zip(arrays, ("dq", "dk", "dv")):
+            value, bound = want[name]  # the cotangent itself is rounded once more on the way
+            within(a.grad().to_numpy(), (value, bound + 4 * U * np.abs(bound).max() + 8 * U * np.abs(value)), name)
+
+
+@pytest.mark.gpu
 def test_two_captured_steps_share_nothing():
     """Two captured steps of different sizes, replayed in turn, and eager calls between them."""
     import endia_amd as nd
