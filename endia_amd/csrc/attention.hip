@@ -14,25 +14,6 @@ using namespace attention;
 
 namespace {
 
-// Pooled memory for the time of one call: work on the one stream is ordered, so it can go back at once.
-struct Scratch {
-  void* p = nullptr;
-  int64_t used = 0;
-  ~Scratch() {
-    if (p) endia_hip_free(p);
-  }
-  int64_t want(int64_t bytes) {  // offset of a piece
-    const int64_t at = used;
-    used += (bytes + 255) / 256 * 256;
-    return at;
-  }
-  int32_t get() { return endia_hip_malloc(used, &p); }
-  template <typename T>
-  T* at(int64_t offset) const {
-    return reinterpret_cast<T*>(static_cast<char*>(p) + offset);
-  }
-};
-
 void make_buckets(const endia_hip_attention_desc* d, Buckets* t) {
   t->both = d->both_sides;
   t->side = d->both_sides ? d->buckets / 2 : d->buckets;

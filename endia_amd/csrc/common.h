@@ -64,3 +64,27 @@ int32_t static_scratch_init(int device);
   } while (0)
 
 static inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Pooled memory for the time of one call: work on the one stream is ordered, so it can go back at once. Pieces start on 256 bytes.
+// The size is rounded up to an eighth of its power of two, so that calls of many lengths share few sizes of the pool.
+struct Scratch {
+  void* p = nullptr;
+  int64_t used = 0;
+  ~Scratch() {
+    if (p) endia_hip_free(p);
+  }
+  int64_t want(int64_t bytes) {  // offset of a piece
+    const int64_t at = used;
+    used += ceil_div64(bytes, 256) * 256;
+    return at;
+  }
+  int32_t get() {
+    int64_t step = 256;
+    while (step * 16 <= used) step *= 2;
+    return endia_hip_malloc(ceil_div64(used, step) * step, &p);
+  }
+  template <typename T>
+  T* at(int64_t offset) const {
+    return reinterpret_cast<T*>(static_cast<char*>(p) + offset);
+  }
+};

@@ -43,7 +43,7 @@ struct Tile {
   }
 };
 typedef Tile<256> Tile256;
-constexpr int FA = Tile256::FA, FB = Tile256::FB, TPB = Tile256::TPB, STAGE = Tile256::STAGE;
+constexpr int FA = Tile256::FA, FB = Tile256::FB, TPB = Tile256::TPB;  // dz_kernel's
 
 template <int T>
 __device__ __forceinline__ void request(const char* a, const char* b, char* stage, const Tile<T>& t) {

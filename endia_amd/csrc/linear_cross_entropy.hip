@@ -17,22 +17,6 @@ namespace {
 
 constexpr int TPB = 256;
 
-struct Scratch {  // a pooled buffer for the time of one call (work on the one stream is ordered, so it can go back at once)
-  void* p = nullptr;
-  int64_t used = 0;
-  int32_t get() { return endia_hip_malloc(used, &p); }
-  int64_t want(int64_t bytes) {  // offset of a piece
-    const int64_t at = used;
-    used += (bytes + 255) / 256 * 256;
-    return at;
-  }
-  char* at(int64_t offset) const { return static_cast<char*>(p) + offset; }
-  float* f(int64_t offset) const { return reinterpret_cast<float*>(at(offset)); }
-  ~Scratch() {
-    if (p) endia_hip_free(p);
-  }
-};
-
 __device__ __forceinline__ bool left_out(float t) { return t < 0.f; }
 
 // lse per row and the mean loss. A target that is no class (NaN, or V and above) makes the loss NaN.
@@ -58,7 +42,7 @@ __global__ __launch_bounds__(TPB) void loss_kernel(int64_t N, int64_t V, const f
   cnt[threadIdx.x] = kept;
   __syncthreads();
   for (int s = TPB / 2; s; s >>= 1) {
-    if (threadIdx.x < s) {
+    if ((int)threadIdx.x < s) {
       red[threadIdx.x] += red[threadIdx.x + s];
       cnt[threadIdx.x] += cnt[threadIdx.x + s];
     }
@@ -157,15 +141,15 @@ int32_t few_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ld
   const int64_t xp = w.want(lce::plane_bytes(N, D)), st = w.want(8 * tiles * N), run = w.want(12 * N), xa = w.want(4 * N);
   int32_t rc = w.get();
   if (rc) return rc;
-  if (scaled && ((rc = lce::row_amax(W, ldw, !transW, V, D, nullptr, wa, s)) || (rc = lce::row_amax(x, ldx, false, N, D, target, w.f(xa), s)))) return rc;
-  if ((rc = lce::planes(x, ldx, false, N, D, target, scaled ? w.f(xa) : nullptr, w.at(xp), s))) return rc;
-  float *m = w.f(run), *l = m + N, *zt = l + N;
+  if (scaled && ((rc = lce::row_amax(W, ldw, !transW, V, D, nullptr, wa, s)) || (rc = lce::row_amax(x, ldx, false, N, D, target, w.at<float>(xa), s)))) return rc;
+  if ((rc = lce::planes(x, ldx, false, N, D, target, scaled ? w.at<float>(xa) : nullptr, w.at<char>(xp), s))) return rc;
+  float *m = w.at<float>(run), *l = m + N, *zt = l + N;
   lce::Direct a = {};
   a.a = W; a.lda = ldw; a.rows = V; a.k = D;
-  a.planes = w.at(xp); a.N = N; a.parts = 1; a.target = target;
-  a.a_amax = wa; a.x_amax = w.f(xa);
-  a.stats = w.f(st); a.zt = zt;
-  if ((rc = lce::direct_stats(a, transW, s)) || (rc = join_stats(w.f(st), tiles, N, m, l, true, s))) return rc;
+  a.planes = w.at<char>(xp); a.N = N; a.parts = 1; a.target = target;
+  a.a_amax = wa; a.x_amax = w.at<float>(xa);
+  a.stats = w.at<float>(st); a.zt = zt;
+  if ((rc = lce::direct_stats(a, transW, s)) || (rc = join_stats(w.at<float>(st), tiles, N, m, l, true, s))) return rc;
   hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(TPB), 0, s, N, V, target, m, l, zt, lse, loss);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
@@ -184,40 +168,40 @@ int32_t few_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ld
                 xta = w.want(4 * D);
   int32_t rc = w.get();
   if (rc) return rc;
-  if (scaled && ((rc = lce::row_amax(x, ldx, false, N, D, target, w.f(xa), s)) ||
-                 (dW && (rc = lce::row_amax(x, ldx, true, D, N, target, w.f(xta), s)))))
+  if (scaled && ((rc = lce::row_amax(x, ldx, false, N, D, target, w.at<float>(xa), s)) ||
+                 (dW && (rc = lce::row_amax(x, ldx, true, D, N, target, w.at<float>(xta), s)))))
     return rc;
-  if ((rc = lce::planes(x, ldx, false, N, D, target, scaled ? w.f(xa) : nullptr, w.at(xp), s))) return rc;
-  if (dW && (rc = lce::planes(x, ldx, true, D, N, target, scaled ? w.f(xta) : nullptr, w.at(xt), s))) return rc;
+  if ((rc = lce::planes(x, ldx, false, N, D, target, scaled ? w.at<float>(xa) : nullptr, w.at<char>(xp), s))) return rc;
+  if (dW && (rc = lce::planes(x, ldx, true, D, N, target, scaled ? w.at<float>(xta) : nullptr, w.at<char>(xt), s))) return rc;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     const int64_t cols = V - v0 < piece ? V - v0 : piece;
     lce::Direct a = {};
     a.a = W + (transW ? v0 * ldw : v0); a.lda = ldw; a.rows = cols; a.k = D;
-    a.planes = w.at(xp); a.N = N; a.v0 = v0; a.parts = 1; a.target = target; a.lse = lse;
-    a.a_amax = lse + N + 1 + v0; a.x_amax = w.f(xa);
-    a.dz = dW ? w.f(dz) : nullptr;
+    a.planes = w.at<char>(xp); a.N = N; a.v0 = v0; a.parts = 1; a.target = target; a.lse = lse;
+    a.a_amax = lse + N + 1 + v0; a.x_amax = w.at<float>(xa);
+    a.dz = dW ? w.at<float>(dz) : nullptr;
     a.dz_ld = cols;
-    a.dz_planes = dx ? w.at(zp) : nullptr;
+    a.dz_planes = dx ? w.at<char>(zp) : nullptr;
     a.g = g; a.count = lse + N;
     if ((rc = lce::direct_dz(a, transW, s))) return rc;
     if (dx) {
       a.rows = D; a.k = cols;
-      a.planes = w.at(zp);
+      a.planes = w.at<char>(zp);
       a.parts = parts;
-      a.out = parts > 1 ? w.f(dxp) : dx;
+      a.out = parts > 1 ? w.at<float>(dxp) : dx;
       a.accumulate = v0 ? 1 : 0;
       if ((rc = lce::direct_dx(a, !transW, s))) return rc;
     }
     if (dW) {
       lce::Outer o = {};
-      o.planes = w.at(xt); o.x_amax = scaled ? w.f(xta) : nullptr; o.dz = w.f(dz); o.dz_ld = cols; o.N = N; o.D = D; o.cols = cols;
+      o.planes = w.at<char>(xt); o.x_amax = scaled ? w.at<float>(xta) : nullptr; o.dz = w.at<float>(dz); o.dz_ld = cols; o.N = N; o.D = D; o.cols = cols;
       o.out = transW ? dW + v0 * D : dW + v0;
       o.ld = transW ? D : V;
       o.g = g; o.count = lse + N;
       if ((rc = lce::direct_dw(o, !transW, s))) return rc;
     }
   }
-  return dx && parts > 1 ? add_parts(w.f(dxp), N, D, parts, dx, D, s) : ENDIA_HIP_OK;
+  return dx && parts > 1 ? add_parts(w.at<float>(dxp), N, D, parts, dx, D, s) : ENDIA_HIP_OK;
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------
@@ -238,17 +222,17 @@ int32_t many_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
   const int64_t xp = w.want(lce::panel_bytes(N, D)), wp = w.want(lce::panel_bytes(piece, D)), xa = w.want(4 * N),
                 st = w.want(8 * tiles * N), run = w.want(12 * N);
   int32_t rc = w.get();
-  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), false, s))) return rc;
-  float *m = w.f(run), *l = m + N, *zt = l + N;
+  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at<char>(xp), w.at<float>(xa), false, s))) return rc;
+  float *m = w.at<float>(run), *l = m + N, *zt = l + N;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     const int64_t cols = V - v0 < piece ? V - v0 : piece;
-    if ((rc = lce::pack(W + (transW ? v0 * ldw : v0), ldw, !transW, cols, D, nullptr, w.at(wp), lse + N + 1 + v0, false, s))) return rc;
+    if ((rc = lce::pack(W + (transW ? v0 * ldw : v0), ldw, !transW, cols, D, nullptr, w.at<char>(wp), lse + N + 1 + v0, false, s))) return rc;
     lce::Logits a = {};
-    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = lse + N + 1 + v0; a.x_amax = w.f(xa); a.target = target;
+    a.w = w.at<char>(wp); a.x = w.at<char>(xp); a.w_amax = lse + N + 1 + v0; a.x_amax = w.at<float>(xa); a.target = target;
     a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
-    a.stats = w.f(st); a.zt = zt;
+    a.stats = w.at<float>(st); a.zt = zt;
     if ((rc = lce::logits_stats(a, s))) return rc;
-    if ((rc = join_stats(w.f(st), ceil_div64(cols, lce::product_tile(cols, N)), N, m, l, v0 == 0, s))) return rc;
+    if ((rc = join_stats(w.at<float>(st), ceil_div64(cols, lce::product_tile(cols, N)), N, m, l, v0 == 0, s))) return rc;
   }
   hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(TPB), 0, s, N, V, target, m, l, zt, lse, loss);
   ENDIA_LAUNCH_CHECK();
@@ -271,34 +255,34 @@ int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
                 ps = w.want(4 * ptiles * rows), pts = w.want(4 * rows / lce::kPanel * ptiles * lce::kPanel),
                 dxp = w.want(dx && parts > 1 ? 4 * parts * N * D : 0), dwp = w.want(dW && w_parts > 1 ? 4 * w_parts * piece * D : 0);
   int32_t rc = w.get();
-  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at(xp), w.f(xa), false, s))) return rc;
-  if (dW && (rc = lce::pack(x, ldx, true, D, N, target, w.at(xt), w.f(xta), false, s))) return rc;
+  if (rc || (rc = lce::pack(x, ldx, false, N, D, target, w.at<char>(xp), w.at<float>(xa), false, s))) return rc;
+  if (dW && (rc = lce::pack(x, ldx, true, D, N, target, w.at<char>(xt), w.at<float>(xta), false, s))) return rc;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     const int64_t cols = V - v0 < piece ? V - v0 : piece;
     const float* Wv = W + (transW ? v0 * ldw : v0);
-    if ((rc = lce::pack(Wv, ldw, !transW, cols, D, nullptr, w.at(wp), const_cast<float*>(lse) + N + 1 + v0, true, s))) return rc;
+    if ((rc = lce::pack(Wv, ldw, !transW, cols, D, nullptr, w.at<char>(wp), const_cast<float*>(lse) + N + 1 + v0, true, s))) return rc;
     lce::Logits a = {};
-    a.w = w.at(wp); a.x = w.at(xp); a.w_amax = lse + N + 1 + v0; a.x_amax = w.f(xa); a.target = target;
+    a.w = w.at<char>(wp); a.x = w.at<char>(xp); a.w_amax = lse + N + 1 + v0; a.x_amax = w.at<float>(xa); a.target = target;
     a.N = N; a.cols = cols; a.v0 = v0; a.D = D;
     a.lse = lse;
-    a.p = dx ? w.at(p) : nullptr;
-    a.pt = dW ? w.at(pt) : nullptr;
-    a.p_shift = reinterpret_cast<int*>(w.at(ps));
-    a.pt_shift = reinterpret_cast<int*>(w.at(pts));
+    a.p = dx ? w.at<char>(p) : nullptr;
+    a.pt = dW ? w.at<char>(pt) : nullptr;
+    a.p_shift = w.at<int>(ps);
+    a.pt_shift = w.at<int>(pts);
     if ((rc = lce::logits_dz(a, s))) return rc;
     lce::Gradient q = {};
     q.g = g;
     q.count = lse + N;
     if (dx) {
-      if ((rc = lce::pack(Wv, ldw, transW, D, cols, nullptr, w.at(wt), w.f(wta), false, s))) return rc;
-      q.a = w.at(wt); q.b = a.p; q.a_amax = w.f(wta); q.b_shift = a.p_shift; q.b_shift_ld = rows;
+      if ((rc = lce::pack(Wv, ldw, transW, D, cols, nullptr, w.at<char>(wt), w.at<float>(wta), false, s))) return rc;
+      q.a = w.at<char>(wt); q.b = a.p; q.a_amax = w.at<float>(wta); q.b_shift = a.p_shift; q.b_shift_ld = rows;
       q.rows_a = D; q.rows_b = N; q.k = cols;
-      q.out = parts > 1 ? w.f(dxp) : dx;
+      q.out = parts > 1 ? w.at<float>(dxp) : dx;
       q.ld = D; q.by_a = 0; q.accumulate = v0 ? 1 : 0; q.parts = parts; q.part_stride = N * D;
       if ((rc = lce::gradient(q, s))) return rc;
     }
     if (dW) {
-      q.a = w.at(xt); q.b = a.pt; q.a_amax = w.f(xta); q.b_shift = a.pt_shift; q.b_shift_ld = ceil_div64(cols, lce::kPanel) * lce::kPanel;
+      q.a = w.at<char>(xt); q.b = a.pt; q.a_amax = w.at<float>(xta); q.b_shift = a.pt_shift; q.b_shift_ld = ceil_div64(cols, lce::kPanel) * lce::kPanel;
       q.rows_a = D; q.rows_b = cols; q.k = N;
       q.out = transW ? dW + v0 * D : dW + v0;
       q.ld = transW ? D : V;
@@ -306,14 +290,14 @@ int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
       float* out = q.out;
       const int64_t ld = q.ld;
       if (w_parts > 1) {
-        q.out = w.f(dwp);
+        q.out = w.at<float>(dwp);
         q.ld = transW ? D : cols;
       }
       if ((rc = lce::gradient(q, s))) return rc;
       if (w_parts > 1 && (rc = add_parts(q.out, transW ? cols : D, transW ? D : cols, w_parts, out, ld, s))) return rc;
     }
   }
-  return dx && parts > 1 ? add_parts(w.f(dxp), N, D, parts, dx, D, s) : ENDIA_HIP_OK;
+  return dx && parts > 1 ? add_parts(w.at<float>(dxp), N, D, parts, dx, D, s) : ENDIA_HIP_OK;
 }
 
 }  // namespace
