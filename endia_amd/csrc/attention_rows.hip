@@ -97,14 +97,13 @@ __global__ __launch_bounds__(TPB) void rows_kernel(Args a) {
         t[u] = j < limit[r] && j < last ? d : -INFINITY;
         top = fmaxf(top, t[u]);
       }
-      if (top == -INFINITY) continue;
       const float keep = carry(m[r], top);
       m[r] = top;
       l[r] *= keep;
       o[r].x *= keep; o[r].y *= keep; o[r].z *= keep; o[r].w *= keep;
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
-        if (t[u] == -INFINITY) continue;  // a key that is left out adds nothing, whatever its row holds
+        if (t[u] == -INFINITY) continue;  // a key that is left out adds nothing, whatever its row holds (a NaN score does: fmaxf drops it from top)
         const float p = exp2_fast(t[u] - top);
         l[r] += p;
         o[r].x += p * vf[u].x; o[r].y += p * vf[u].y; o[r].z += p * vf[u].z; o[r].w += p * vf[u].w;
@@ -129,12 +128,11 @@ __global__ __launch_bounds__(TPB) void rows_kernel(Args a) {
     float top = -INFINITY;
     for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, lds_m[r][g]);
     float sum = 0.f, out = 0.f;
-    if (top > -INFINITY)
-      for (int g = 0; g < GROUPS; ++g) {
-        const float w = carry(lds_m[r][g], top);
-        sum += w * lds_l[r][g];
-        out += w * lds_o[r][g][d];
-      }
+    for (int g = 0; g < GROUPS; ++g) {  // (all maxima -inf: no key, and zeros are joined, or nothing but NaN scores, and NaN are)
+      const float w = carry(lds_m[r][g], top);
+      sum += w * lds_l[r][g];
+      out += w * lds_o[r][g][d];
+    }
     const int64_t h = kh * a.G + row / a.Q, i = row % a.Q;
     if (a.splits == 1) {
       if (d < D) a.o[((b * a.Q + i) * a.H + h) * D + d] = sum != 0.f ? out / sum : 0.f;
@@ -151,7 +149,7 @@ __global__ __launch_bounds__(TPB) void rows_kernel(Args a) {
 }
 
 // One wave per row: joins the parts' outputs, each relative to its part's maximum. The lanes first share the parts' weights out
-// among them.
+// among them. A part whose maximum is -inf has weight 0 and holds zeros (no key) or NaN (nothing but NaN scores), which 0 leaves NaN.
 __global__ __launch_bounds__(TPB) void combine_kernel(Args a) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (b H + h) Q + i
@@ -163,22 +161,21 @@ __global__ __launch_bounds__(TPB) void combine_kernel(Args a) {
   top = wave_max(top);
   float o0 = 0.f, o1 = 0.f;
   const float* part = a.part + row * a.splits * a.D;
-  if (top > -INFINITY)
-    for (int s0 = 0; s0 < a.splits; s0 += 64) {
-      float w = 0.f;
-      if (s0 + lane < a.splits) {
-        const float2 f = ml[s0 + lane];
-        w = carry(f.x, top);
-        sum += w * f.y;
-      }
-      const int n = min(64, a.splits - s0);
-      for (int s = 0; s < n; ++s) {
-        const float ws = __shfl(w, s, 64);
-        const float* from = part + (s0 + s) * a.D;
-        if (lane < a.D) o0 += ws * from[lane];
-        if (lane + 64 < a.D) o1 += ws * from[lane + 64];
-      }
+  for (int s0 = 0; s0 < a.splits; s0 += 64) {
+    float w = 0.f;
+    if (s0 + lane < a.splits) {
+      const float2 f = ml[s0 + lane];
+      w = carry(f.x, top);
+      sum += w * f.y;
     }
+    const int n = min(64, a.splits - s0);
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl(w, s, 64);
+      const float* from = part + (s0 + s) * a.D;
+      if (lane < a.D) o0 += ws * from[lane];
+      if (lane + 64 < a.D) o1 += ws * from[lane + 64];
+    }
+  }
 #pragma unroll
   for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w, 64);
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
