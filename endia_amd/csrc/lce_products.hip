@@ -201,6 +201,13 @@ __global__ __launch_bounds__(Tile<T>::TPB, 2) void stats_kernel(Logits p) {
   }
 }
 
+// The largest shift of a tile's cotangents. gradient_kernel moves its sums from one tile's shift to the next one's, which is upwards
+// where a tile of small cotangents, or of zeros (256 rows that are left out), follows one of large ones. |dz| <= 1 has a shift of at
+// least 13, and the factors of a product are below 2^14. Along the classes a row's |dz| add up to 2 at most: sums below 2^28 that
+// move up by 100 - 13 stay below 2^115. Along the rows there may be N < 2^b of size 1: sums below 2^(28 + b), so shifts up to
+// 111 - b keep them below 2^126. (Up to 2047 rows that is no limit; a class of cotangents all below 2^(b - 98) lies lower in fp16's range.)
+__device__ __forceinline__ int most_shift_of_class(int64_t N) { return min(kMaxShift, 79 + __clz((int)N)); }
+
 // dz = exp(z - lse) - [class = target] (zeros for rows that are left out and behind the ends), stored twice as pairs: rows of x
 // along k for the weight's gradient, classes along k for x's gradient. The scale of a row is one power of two per tile, from the
 // tile's own largest, so that rows that are nearly right and classes that are hardly likely keep their precision.
@@ -260,7 +267,8 @@ __global__ __launch_bounds__(TPB, 2) void dz_kernel(Logits p) {
   int sb[FB];
 #pragma unroll
   for (int j = 0; j < FB; ++j) sb[j] = shift_of(__uint_as_float(row_max[t.b_of(j)]));
-  const int own_shift = shift_of(__uint_as_float(row_max[threadIdx.x]));  // of a row, or of class threadIdx.x - 256
+  int own_shift = shift_of(__uint_as_float(row_max[threadIdx.x]));  // of a row, or of class threadIdx.x - 256
+  if (threadIdx.x >= kPanel) own_shift = min(own_shift, most_shift_of_class(p.N));
   if (threadIdx.x < kPanel) p.p_shift[(int64_t)ta * tiles_b * kPanel + b0 + threadIdx.x] = own_shift;
   else p.pt_shift[(int64_t)tb * tiles_a * kPanel + a0 + threadIdx.x - kPanel] = own_shift;
   __syncthreads();
@@ -365,7 +373,7 @@ __global__ __launch_bounds__(Tile<T>::TPB, 2) void gradient_kernel(Gradient p) {
   wait_loads();
   __syncthreads();
   for (int kb = k0; kb < k1; ++kb) {
-    if ((kb & 7) == 0 && kb != k0) {  // the next 256 of k have scales of their own: the sums so far move to them
+    if ((kb & 7) == 0 && kb != k0) {  // the next 256 of k have scales of their own: the sums so far move to them (see most_shift_of_class)
 #pragma unroll
       for (int j = 0; j < FB; ++j) {
         const int now = shifts[(int64_t)(kb / 8) * p.b_shift_ld + t.b_of(j)];
@@ -382,14 +390,13 @@ __global__ __launch_bounds__(Tile<T>::TPB, 2) void gradient_kernel(Gradient p) {
     wait_loads();
     __syncthreads();
   }
-  const float c = p.count[0] > 0.f ? p.g[0] / p.count[0] : 0.f;
+  const Mean c = mean_of(p.g, p.count);
   float* out = p.out + part * p.part_stride;
   const bool vec = p.vec;
 #pragma unroll
   for (int j = 0; j < FB; ++j) {
     const int64_t bi = b0 + t.b_of(j);
     if (bi >= p.rows_b) continue;
-    const float cb = __builtin_ldexpf(c, -shift[j]);
 #pragma unroll
     for (int i = 0; i < FA; ++i)
 #pragma unroll
@@ -397,7 +404,7 @@ __global__ __launch_bounds__(Tile<T>::TPB, 2) void gradient_kernel(Gradient p) {
         const int64_t ai = a0 + t.a_of(i, 4 * q);
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = acc[i][j][4 * q + e] * (cb * __builtin_ldexpf(1.f, -shift_of(p.a_amax[min(ai + e, p.rows_a - 1)])));
+        for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(acc[i][j][4 * q + e] * c.m, c.e - shift[j] - shift_of(p.a_amax[min(ai + e, p.rows_a - 1)]));
         if (vec) {
           if (ai < p.rows_a) {
             float4* to = reinterpret_cast<float4*>(out + bi * p.ld + ai);

@@ -18,6 +18,18 @@ __device__ __forceinline__ char* line_at(char* panels, int64_t row, int64_t kb, 
   return panels + ((row / kPanel) * kblocks + kb) * kBlockBytes + (row % kPanel) * 128;
 }
 
+// g / count = m 2^e (0 without a row that counts). A result is put together as ldexp(sum * m, e - shifts): the powers of two that
+// scales take off, and a small cotangent, would leave fp32's range as a factor of their own though the result does not.
+struct Mean {
+  float m;
+  int e;
+};
+__device__ __forceinline__ Mean mean_of(const float* g, const float* count) {
+  const float c = g[0], n = count[0];
+  if (!(n > 0.f)) return {0.f, 0};
+  return {__builtin_amdgcn_frexp_mantf(c) / n, __builtin_amdgcn_frexp_expf(c)};  // (infinities and NaN: themselves, 0)
+}
+
 // Source of an operand [rows, k]: element (r, k) at x[r * ld + k], or transposed at x[k * ld + r]. `left_out` (null or one target
 // per index along x's first axis): indices with a negative target are zeros. amax: per row the largest finite magnitude.
 int32_t pack(const float* x, int64_t ld, bool transposed, int64_t rows, int64_t k, const float* left_out, char* panels, float* amax,
@@ -40,7 +52,7 @@ int32_t logits_dz(const Logits& a, hipStream_t s);
 
 // out (+)= c * B A^T: A [rows_a, k] with one scale per row, B [rows_b, k] with one shift per row and 256 of k.
 // element (b, a) at out[b * ld + a], or with by_a at out[a * ld + b]. parts: the walk along k cut into that many; part s goes to
-// out + s * part_stride. c: g[0] / count[0].
+// out + s * part_stride. c: the Mean of g and count.
 struct Gradient {
   const char *a, *b;
   const float* a_amax;

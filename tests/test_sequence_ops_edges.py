@@ -59,3 +59,54 @@ def test_attention_nan_in_a_key_or_value_reaches_every_row(Q, K):
             assert not np.isfinite(o[:, :, 0, 5]).any(), j
             o[:, :, 0, 5] = want[0][:, :, 0, 5]
             within(o, want, "o")
+
+
+# ---- linear_cross_entropy: scales at the ends of the range ------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("N", [513, 768, 8392, 9000])
+def test_linear_cross_entropy_left_out_tail(N, tied):
+    """Padding at the end of the batch: the last rows are left out, whole tiles of 256 among them, alone in their part of the walk or
+    behind other tiles; small cotangents, small rows."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    for left in (N % 256 or 256, 300):
+        for size in (1.0, 1e-3):
+            x, w = (size * rng.standard_normal((N, 40))).astype(np.float32), (rng.standard_normal((40, 333)) / 6).astype(np.float32)
+            t = rng.integers(0, 333, N).astype(np.float32)
+            t[N - left:] = -1
+            for g in (1.0, 1e-4, 1e-8):
+                want, got = loss_reference(x, w, t, g), loss_of(nd, x, w, t, tied, g=g)
+                for n in got:
+                    within(got[n], want[n], "%s with %d of %d left out, size %g, cotangent %g" % (n, left, N, size, g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [False, True])
+def test_linear_cross_entropy_long_sums_before_left_out_rows(tied):
+    """A million rows that are all wrong about one class, in a column of x that never changes its sign: sums of 2^16 such rows, and
+    then 256 rows that are left out."""
+    import endia_amd as nd
+    N = (1 << 20) + 256
+    x = np.full((N, 2), 1.99, np.float32)
+    x[:, 1] = np.random.default_rng(0).standard_normal(N)
+    w = np.array([[-8, 8, 0], [0.1, 0.2, 0.3]], np.float32)
+    t = np.zeros(N, np.float32)
+    t[1 << 20:] = -1
+    want, got = loss_reference(x, w, t), loss_of(nd, x, w, t, tied)
+    for n in got:
+        within(got[n], want[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("N", [600])
+def test_linear_cross_entropy_of_a_tiny_cotangent(N, tied):
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal((N, 40)).astype(np.float32), (rng.standard_normal((40, 333)) / 6).astype(np.float32)
+    t = rng.integers(0, 333, N).astype(np.float32)
+    for g in (1e-20, -1e-30, 1e20):
+        want, got = loss_reference(x, w, t, g), loss_of(nd, x, w, t, tied, g=g)
+        for n in got:
+            within(got[n], want[n], "%s with a cotangent of %g" % (n, g))
