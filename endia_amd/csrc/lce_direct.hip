@@ -201,14 +201,26 @@ __device__ __forceinline__ void dz_block(const Direct& p, const floatx16& acc, i
       }
 }
 
+// sum 2^-kUp g / count as sum * a * b, neither of which leaves fp32's range
+struct Down {
+  float a, b;
+  __device__ __forceinline__ explicit Down(const Mean& c) {
+    const int e = c.e - kUp, h = e / 2;
+    a = __builtin_ldexpf(c.m, h);
+    b = __builtin_ldexpf(1.f, e - h);
+  }
+  __device__ __forceinline__ float operator()(float sum) const { return sum * a * b; }
+};
+
 __device__ __forceinline__ void dx_block(const Direct& p, const floatx16& acc, int64_t r0, int left, int n, int half, int part) {
   if (n >= p.N) return;
-  const float c = p.count[0] > 0.f ? __builtin_ldexpf(p.g[0] / p.count[0], -kUp) : 0.f;
+  const Down down(mean_of(p.g, p.count));
   float* out = p.out + ((int64_t)part * p.N + n) * p.rows + r0;
 #pragma unroll
   for (int v = 0; v < 16; ++v) {
     const int i = k_of(half, v & 7) + 16 * (v >> 3);
-    if (i < left) out[i] = p.accumulate ? out[i] + acc[v] * c : acc[v] * c;
+    const float y = down(acc[v]);
+    if (i < left) out[i] = p.accumulate ? out[i] + y : y;
   }
 }
 
@@ -384,7 +396,8 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
   const int64_t v0 = (int64_t)blockIdx.x * 128 + wave * 32, v = v0 + col;
   const int steps = (int)((p.N + 15) / 16), chunks = (steps + CS - 1) / CS, blocks = (int)((p.D + 31) / 32);
   const int groups = (blocks + DB - 1) / DB, g0 = blockIdx.y * p.groups, g1 = min(g0 + p.groups, groups);
-  const float c = p.count[0] > 0.f ? __builtin_ldexpf(p.g[0] / p.count[0], -kUp) : 0.f;
+  const Mean c = mean_of(p.g, p.count);
+  const Down down(c);
   const int turns = (g1 - g0) * chunks;
   auto request = [&](int turn, char* to) {
     const int g = g0 + turn / chunks, ch = turn % chunks;
@@ -442,22 +455,22 @@ __global__ __launch_bounds__(TPB, 2) void outer_kernel(Outer p) {
     if (turn % chunks == chunks - 1) {
       const int d0 = (g0 + turn / chunks) * DB * 32;
       // The axis that lies contiguous in the output is the one along the lanes. (Pairs: the scales come off, of the lane's class and
-      // of x's columns; with classes along the registers, lane k has those of class k.)
-      const float down_v = P == 2 ? __builtin_ldexpf(c, -shift) : c;
+      // of x's columns, the latter with 2^-kUp; with classes along the registers, lane k has those of class k.)
+      const float down_v = __builtin_ldexpf(c.m, c.e - shift);
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
-        const float down_lane = P == 2 && !BY_D ? __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min(d0 + b * 32 + col, (int)p.D - 1)])) : 1.f;
+        const float down_lane = P == 2 && !BY_D ? __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min(d0 + b * 32 + col, (int)p.D - 1)]) - kUp) : 1.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int k = k_of(half, i & 7) + 16 * (i >> 3);
           if (BY_D) {
             const int d = d0 + b * 32 + k;
-            const float down = P == 2 ? __builtin_ldexpf(down_v, -pairs::shift_of(p.x_amax[min(d, (int)p.D - 1)])) : down_v;
-            if (v < p.cols && d < p.D) p.out[(int64_t)d * p.ld + v] = acc[b][i] * down;
+            const float down_d = P == 2 ? __builtin_ldexpf(1.f, -pairs::shift_of(p.x_amax[min(d, (int)p.D - 1)]) - kUp) : 1.f;
+            if (v < p.cols && d < p.D) p.out[(int64_t)d * p.ld + v] = P == 2 ? acc[b][i] * down_v * down_d : down(acc[b][i]);
           } else {
             const int d = d0 + b * 32 + col;
-            const float down = P == 2 ? down_lane * __shfl(down_v, k, 64) : c;
-            if (d < p.D && v0 + k < p.cols) p.out[(v0 + k) * p.ld + d] = acc[b][i] * down;
+            const float down_k = P == 2 ? __shfl(down_v, k, 64) : 1.f;
+            if (d < p.D && v0 + k < p.cols) p.out[(v0 + k) * p.ld + d] = P == 2 ? acc[b][i] * down_k * down_lane : down(acc[b][i]);
           }
         }
         __builtin_amdgcn_sched_barrier(0);

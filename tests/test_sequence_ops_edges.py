@@ -100,7 +100,7 @@ def test_linear_cross_entropy_long_sums_before_left_out_rows(tied):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tied", [False, True])
-@pytest.mark.parametrize("N", [600])
+@pytest.mark.parametrize("N", [9, 90, 600])
 def test_linear_cross_entropy_of_a_tiny_cotangent(N, tied):
     import endia_amd as nd
     rng = np.random.default_rng(0)
