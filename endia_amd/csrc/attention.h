@@ -34,6 +34,8 @@ struct Args {
   int64_t B, Q, K, H, Hk, D, G;
   int64_t qs[3], ks[3], vs[3];
   int64_t off;
+  int64_t seen;  // keys that any query sees: K, or with causal those before Q + off. What a cache holds behind them takes no part in
+                 // a tile's scale, in a product or in a gradient.
   float scale;
   int causal;
   int vec;  // q, k, v (and o, go, which are contiguous) can be read 16 bytes at a time
@@ -55,9 +57,9 @@ struct Args {
 };
 
 __device__ __forceinline__ int key_count(const Args& a, int64_t b) {
-  if (!a.lengths) return (int)a.K;
+  if (!a.lengths) return (int)a.seen;
   const float n = a.lengths[b];
-  return n > 0.f ? (n < (float)a.K ? (int)n : (int)a.K) : 0;
+  return n > 0.f ? (n < (float)a.seen ? (int)n : (int)a.seen) : 0;
 }
 
 // Work-groups are dealt round-robin to the 8 XCDs, each with an L2 of its own: give every XCD a contiguous range of ids, so

@@ -68,6 +68,8 @@ Args make_args(const endia_hip_attention_desc* d, const float* q, const float* k
   a.off = d->query_offset;
   a.scale = d->scale;
   a.causal = d->causal ? 1 : 0;
+  a.seen = d->K;
+  if (a.causal && d->Q + d->query_offset < a.seen) a.seen = d->Q + d->query_offset > 0 ? d->Q + d->query_offset : 0;
   a.q = q; a.k = k; a.v = v; a.lengths = lengths; a.table = table;
   a.vec = d->D % 4 == 0 && on16(q, d->q_strides) && on16(k, d->k_strides) && on16(v, d->v_strides);
   a.splits = 1;

@@ -61,6 +61,41 @@ def test_attention_nan_in_a_key_or_value_reaches_every_row(Q, K):
             within(o, want, "o")
 
 
+# ---- attention: keys and queries that the causal mask leaves without a partner -----------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("buckets", [None, 16])
+@pytest.mark.parametrize("Q", [1, 4, 17, 130])
+def test_attention_keys_behind_the_last_query(Q, buckets):
+    """A chunk of queries in a cache with room: what the slots behind the last query hold (NaN, infinities, values that would take a
+    common scale) is never looked at, and their gradients are zeros."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    for offset, K in ((40, Q + 90), (0, Q + 5), (300, Q + 333)):
+        q, k, v, go = (rng.standard_normal((2, n, 2, 64)).astype(np.float32) for n in (Q, K, K, Q))
+        table = rng.standard_normal((buckets, 2)).astype(np.float32) if buckets else None
+        kw = dict(table=table, causal=True, offset=offset, max_distance=32)
+        want = attention_reference(q, k, v, go, **kw)
+        seen = Q + offset
+        for ends in ((np.nan, np.inf), (1e30, -1e30), (-np.inf, np.nan)):
+            k[:, seen:], v[:, seen:] = ends
+            got = attend(nd, q, k, v, go, **kw)
+            for n in want:
+                within(got[n], want[n], "%s at offset %d" % (n, offset))
+            assert not got["dk"][:, seen:].any() and not got["dv"][:, seen:].any()
+
+
+@pytest.mark.gpu
+def test_attention_causal_before_the_first_key():
+    """All queries stand before the first key."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    for Q, offset in ((3, -3), (3, -1000), (70, -70), (70, -100000)):
+        q, k, v, go = (rng.standard_normal((1, n, 2, 32)).astype(np.float32) for n in (Q, 40, 40, Q))
+        k[:], v[:] = np.nan, np.inf
+        got = attend(nd, q, k, v, go, causal=True, offset=offset)
+        assert not any(got[n].any() for n in NAMES), (Q, offset)
+
+
 # ---- linear_cross_entropy: scales at the ends of the range ------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("tied", [False, True])
