@@ -5,7 +5,7 @@
 // of 128 bytes: 32 hi, 32 lo; its column image one line per element of the head dimension: the 32 positions' hi, then lo,
 // with the positions in the order in which an accumulator of the 32 x 32 product holds its rows (see the order below), so
 // that a product of probabilities can take them from the accumulator registers as they are. One shift per tile.
-// Bound: HBM. Reads 4 and writes 4 or 8 bytes per element; positions behind a sequence's length become zeros. Measured: 36 us on
+// Bound: HBM. Reads 4 and writes 4 or 8 bytes per element; keys that no query sees and queries that see no key become zeros. Measured: 36 us on
 // average for the three launches of a step over 8 x 448 queries and 8 x 1500 keys of 16 heads of 64 (0.49 GB in all: 4.5 TB/s).
 #include "attention.h"
 
@@ -18,7 +18,8 @@ constexpr int TPB = 256;
 struct Source {
   const float* x;
   int64_t sb, sp, sh, L, H;
-  int use_lengths;
+  int64_t first;    // positions before it become zeros: queries that see no key
+  int use_lengths;  // so do those behind the sequence's keys
   char *rows, *cols;
   int* shift;
   const float *o, *lse;  // with meta: the forward pass's output and lse beside go = x
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(TPB) void tiles_kernel(Args a, Source s0, Source s1
   for (int i = 0; i < ITEMS; ++i) {
     const int item = tid + i * TPB, row = item / PER_ROW, ch = item % PER_ROW;
     const int64_t p = tile * kTile + row;
-    const bool in = item < 32 * PER_ROW && p < n;
+    const bool in = item < 32 * PER_ROW && p >= src.first && p < n;
     const float* base = src.x + b * src.sb + min(p, src.L - 1) * src.sp + h * src.sh;
     float dot = 0.f;
 #pragma unroll
@@ -132,12 +133,13 @@ int32_t launch(const Args& a, int DP, const Source& s0, const Source& s1, hipStr
 }  // namespace
 
 int32_t launch_tiles(const Args& a, int DP, bool backward, hipStream_t s) {
-  const Source k = {a.k, a.ks[0], a.ks[1], a.ks[2], a.K, a.Hk, 1, a.k_rows, a.k_cols, a.k_shift, nullptr, nullptr, nullptr};
-  const Source v = {a.v, a.vs[0], a.vs[1], a.vs[2], a.K, a.Hk, 1, a.v_rows, a.v_cols, a.v_shift, nullptr, nullptr, nullptr};
+  const Source k = {a.k, a.ks[0], a.ks[1], a.ks[2], a.K, a.Hk, 0, 1, a.k_rows, a.k_cols, a.k_shift, nullptr, nullptr, nullptr};
+  const Source v = {a.v, a.vs[0], a.vs[1], a.vs[2], a.K, a.Hk, 0, 1, a.v_rows, a.v_cols, a.v_shift, nullptr, nullptr, nullptr};
   int32_t rc = launch(a, DP, k, v, s);
   if (rc || !backward) return rc;
-  const Source q = {a.q, a.qs[0], a.qs[1], a.qs[2], a.Q, a.H, 0, a.q_rows, a.q_cols, a.q_shift, nullptr, nullptr, nullptr};
-  const Source g = {a.go, a.Q * a.H * a.D, a.H * a.D, a.D, a.Q, a.H, 0, a.g_rows, a.g_cols, a.g_shift, a.out, a.lse, a.meta};
+  const int64_t first = a.causal && a.off < 0 ? -a.off : 0;
+  const Source q = {a.q, a.qs[0], a.qs[1], a.qs[2], a.Q, a.H, first, 0, a.q_rows, a.q_cols, a.q_shift, nullptr, nullptr, nullptr};
+  const Source g = {a.go, a.Q * a.H * a.D, a.H * a.D, a.D, a.Q, a.H, first, 0, a.g_rows, a.g_cols, a.g_shift, a.out, a.lse, a.meta};
   return launch(a, DP, q, g, s);
 }
 

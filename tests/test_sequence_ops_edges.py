@@ -96,6 +96,25 @@ def test_attention_causal_before_the_first_key():
         assert not any(got[n].any() for n in NAMES), (Q, offset)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("Q, K", [(20, 40), (100, 90), (200, 40)])
+def test_attention_queries_without_a_key_pass_nothing_on(Q, K):
+    """What stands in a query, or comes as the cotangent of one, that sees no key reaches no gradient."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    for none in (1, Q // 2 + 3):
+        q, k, v, go = (rng.standard_normal((1, n, 2, 64)).astype(np.float32) for n in (Q, K, K, Q))
+        table = rng.standard_normal((16, 2)).astype(np.float32)
+        kw = dict(table=table, causal=True, offset=-none, max_distance=32)
+        want = attention_reference(q, k, v, go, **kw)
+        for values in ((np.nan, np.nan), (np.inf, 1e30), (1e30, -np.inf)):
+            q[:, :none], go[:, :none] = values
+            got = attend(nd, q, k, v, go, **kw)
+            for n in want:
+                within(got[n], want[n], n)
+            assert not got["dq"][:, :none].any()
+
+
 # ---- linear_cross_entropy: scales at the ends of the range ------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("tied", [False, True])
