@@ -1361,12 +1361,13 @@ def linear_cross_entropy(x, weight, target):
     def vjp(primals, grad, out_):
         _first_order_only("linear_cross_entropy", grad, out_)
         px, pw, _ = primals
+        g = contiguous(grad)
         dx = Array.empty(px._shape) if px._requires_grad else None
         dw = Array.empty([V, D] if trans else [D, V]) if pw._requires_grad else None
         if dx is None and dw is None:
             return [None, None, None]
         L.call("endia_hip_linear_cross_entropy_bwd", N, D, V, xs.data_ptr(), D, trans, ws.data_ptr(), ldw, ts.data_ptr(), lse.data_ptr(),
-               contiguous(grad).data_ptr(), dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None)
+               g.data_ptr(), dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None)
         if dw is not None and trans:  # the gradient of a transposed view, as a transposed view
             dw = Array([D, V], _buffer=dw._buf, _strides=[1, D])
         return [dx, dw, None]
@@ -1413,10 +1414,11 @@ def _attention(name, q, k, v, table, key_lengths, causal, scale, query_offset, m
 
     def vjp(primals, grad, out_):
         _first_order_only(name, grad, out_)
+        g = contiguous(grad)  # (held until the call is made: a copy that dies before it would be free memory during it)
         grads = [Array.empty(p._shape) if p._requires_grad else None for p in primals]
         dtable = grads[3] if table is not None else None
         L.call("endia_hip_attention_bwd", ctypes.byref(desc), qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), ptr(lens), ptr(tab), out_.data_ptr(),
-               lse.data_ptr(), contiguous(grad).data_ptr(), ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(dtable))
+               lse.data_ptr(), g.data_ptr(), ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(dtable))
         return grads
 
     return _register(out, args, name, vjp)

@@ -115,6 +115,25 @@ def test_attention_queries_without_a_key_pass_nothing_on(Q, K):
             assert not got["dq"][:, :none].any()
 
 
+# ---- attention: memory ----------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_attention_holds_the_cotangent_through_the_call(monkeypatch):
+    """A cotangent that is spread out (a mean's) is copied for the call; the copy lives until the call has been made."""
+    import endia_amd as nd
+    from endia_amd import _array, _lib
+    call, held = _lib.call, []
+
+    def watch(name, *args):
+        if name == "endia_hip_attention_bwd":
+            held.append(not any(args[8] in free for free in _array._FREE.values()))
+        return call(name, *args)
+
+    monkeypatch.setattr(_lib, "call", watch)
+    x = nd.ones([2, 20, 2, 32], requires_grad=True)
+    nd.mean(nd.attention(x, x, x)).backward()
+    assert held == [True]
+
+
 # ---- linear_cross_entropy: scales at the ends of the range ------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("tied", [False, True])
