@@ -30,6 +30,12 @@ __device__ __forceinline__ int bucket_of(const Buckets& t, int rel) {
   return base + (n < t.exact ? n : i);
 }
 
+// Of one tile of 32 positions: its shift, and a bit for each position that holds an infinity or NaN.
+struct TileInfo {
+  int shift;
+  unsigned bad;
+};
+
 struct Args {
   int64_t B, Q, K, H, Hk, D, G;
   int64_t qs[3], ks[3], vs[3];
@@ -43,9 +49,9 @@ struct Args {
   const float *out, *go;  // backward
   float *o, *lse;
   float *dq, *dk, *dv;
-  // tile images of split operands (see prepare_tiles) and the shifts of their tiles
+  // tile images of split operands (see tiles_kernel) and what is known of their tiles
   char *k_rows, *k_cols, *v_rows, *v_cols, *q_rows, *q_cols, *g_rows, *g_cols;
-  int *k_shift, *v_shift, *q_shift, *g_shift;
+  TileInfo *k_info, *v_info, *q_info, *g_info;
   float* meta;       // per query tile: 32 x lse (base 2), 32 x delta
   float* part;       // partial results of a split walk
   float* part_ml;    // forward: running maximum (base 2) and sum of each partial result
@@ -140,6 +146,15 @@ __device__ __forceinline__ void read_line(const char* lines, int line, int s, in
   const char* at = lines + line * 128;
   hi = *reinterpret_cast<const pairs::half8*>(at + (((2 * s + h) ^ (line & 7)) << 4));
   lo = *reinterpret_cast<const pairs::half8*>(at + (((4 + 2 * s + h) ^ (line & 7)) << 4));
+}
+
+// An infinity or NaN in v (or do) has to reach the rows that see it, but in a product with p = 0 it would also reach those of its tile
+// that do not. So the column images hold zeros in its place, and where a tile has any, they are put into the results behind the walk:
+// what `row` holds of them makes the lane's part of `out` NaN. (k and q need this not: they make ds NaN where they are seen.)
+__device__ __forceinline__ void put_bad(const float* row, int D, int half, float* out) {
+  for (int d = 4 * half; d < D; d += 8)
+    for (int at = d; at < min(d + 4, D); ++at)
+      if (!(__builtin_fabsf(row[at]) < INFINITY)) out[at] = NAN;
 }
 
 // score bias of one head by position difference, -near .. near, in LDS, base 2

@@ -123,13 +123,13 @@ int32_t endia_hip_attention_fwd(const endia_hip_attention_desc* d, const float* 
   const int64_t tiles = ceil_div64(a.K, kTile), images = a.B * a.Hk * tiles * DP * 128;
   a.splits = parts(ceil_div64(a.Q, 128) * a.H * a.B, cus, tiles, 4);
   const int64_t n = a.splits > 1 ? a.B * a.H * a.Q * a.splits : 0;
-  const int64_t kr = w.want(images), vc = w.want(images), ks = w.want(4 * a.B * a.Hk * tiles), vs = w.want(4 * a.B * a.Hk * tiles),
+  const int64_t kr = w.want(images), vc = w.want(images), ks = w.want(sizeof(TileInfo) * a.B * a.Hk * tiles), vs = w.want(sizeof(TileInfo) * a.B * a.Hk * tiles),
                 part = w.want(4 * n * a.D), ml = w.want(8 * n);
   if ((rc = w.get())) return rc;
   a.k_rows = w.at<char>(kr);
   a.v_cols = w.at<char>(vc);
-  a.k_shift = w.at<int>(ks);
-  a.v_shift = w.at<int>(vs);
+  a.k_info = w.at<TileInfo>(ks);
+  a.v_info = w.at<TileInfo>(vs);
   a.part = w.at<float>(part);
   a.part_ml = w.at<float>(ml);
   if ((rc = launch_tiles(a, DP, false, st))) return rc;
@@ -161,8 +161,8 @@ int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* 
   ak.splits = parts(ceil_div64(a.K, 128) * a.Hk * a.B, cus, a.G * qt, 4);
   Scratch w;
   const int64_t kr = w.want(kn * image), kc = w.want(kn * image), vr = w.want(kn * image), qr = w.want(qn * image), qc = w.want(qn * image),
-                gr = w.want(qn * image), gc = w.want(qn * image), ksh = w.want(4 * kn), vsh = w.want(4 * kn), qsh = w.want(4 * qn),
-                gsh = w.want(4 * qn), meta = w.want(256 * qn);
+                gr = w.want(qn * image), gc = w.want(qn * image), ki = w.want(sizeof(TileInfo) * kn), vi = w.want(sizeof(TileInfo) * kn),
+                qi = w.want(sizeof(TileInfo) * qn), gi = w.want(sizeof(TileInfo) * qn), meta = w.want(256 * qn);
   const int64_t part_q = aq.splits > 1 ? 4 * aq.splits * a.B * a.Q * a.H * a.D : 0, part_k = ak.splits > 1 ? 8 * ak.splits * a.B * a.K * a.Hk * a.D : 0;
   const int64_t part = w.want(part_q > part_k ? part_q : part_k);  // (one after the other on the stream)
   const int64_t span = 2 * a.bk.near + 1, table_part = w.want(dtable ? table_groups(aq) * span * 4 : 0), diff = w.want(dtable ? 8 * a.H * span : 0),
@@ -171,7 +171,7 @@ int32_t endia_hip_attention_bwd(const endia_hip_attention_desc* d, const float* 
   for (Args* x : {&a, &aq, &ak}) {
     x->k_rows = w.at<char>(kr); x->k_cols = w.at<char>(kc); x->v_rows = w.at<char>(vr); x->q_rows = w.at<char>(qr);
     x->q_cols = w.at<char>(qc); x->g_rows = w.at<char>(gr); x->g_cols = w.at<char>(gc);
-    x->k_shift = w.at<int>(ksh); x->v_shift = w.at<int>(vsh); x->q_shift = w.at<int>(qsh); x->g_shift = w.at<int>(gsh);
+    x->k_info = w.at<TileInfo>(ki); x->v_info = w.at<TileInfo>(vi); x->q_info = w.at<TileInfo>(qi); x->g_info = w.at<TileInfo>(gi);
     x->meta = w.at<float>(meta);
     x->part = w.at<float>(part);
     x->part_table = dtable ? w.at<float>(table_part) : nullptr;

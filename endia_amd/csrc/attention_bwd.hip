@@ -81,7 +81,7 @@ __device__ __forceinline__ float far_part(float ds, float p, float p_all, float 
 }
 
 template <int DP, bool BIAS>
-__global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const int* __restrict__ k_shift, const int* __restrict__ v_shift,
+__global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const TileInfo* __restrict__ k_info, const TileInfo* __restrict__ v_info,
                                                                    const float* __restrict__ meta) {
   constexpr int STAGE = DP * 384;  // row images of k and v, column image of k
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int stage = ahead ? (t - t0) & 1 : 0;
-    const int ks = k_shift[tile_at + t], vs = v_shift[tile_at + t];
+    const int ks = k_info[tile_at + t].shift, vs = v_info[tile_at + t].shift;
     if (ahead && t + 1 < t1) request(t + 1, stage ^ 1);
     const char* kimg = smem + stage * STAGE;
     const char* vimg = kimg + DP * 128;
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dq_kernel(Args a, const
 }
 
 template <int DP, bool BIAS>
-__global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, const int* __restrict__ q_shift, const int* __restrict__ g_shift,
+__global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, const TileInfo* __restrict__ q_info, const TileInfo* __restrict__ g_info,
                                                                     const float* __restrict__ meta) {
   constexpr int STAGE = DP * 512 + 256;  // row and column images of q and do; lse and delta
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -347,13 +347,15 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
   for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = floatx16{};
   int FK = 2 * kMaxShift, FV = 2 * kMaxShift;
   int64_t bias_head = -1;
+  unsigned bad = 0;
   if (u0 < u1) request(u0, 0);
   wait_loads();
   __syncthreads();
   for (int u = u0; u < u1; ++u) {
     const int stage = (u - u0) & 1;
     const int64_t t = tile_of(u);
-    const int qs = q_shift[t], gs = g_shift[t];
+    const int qs = q_info[t].shift, gs = g_info[t].shift;
+    bad |= g_info[t].bad;
     if (u + 1 < u1) request(u + 1, stage ^ 1);
     if (BIAS && bias_head != u / each) {  // (uniform over the work-group; everybody is behind the barrier of the last turn)
       bias_head = u / each;
@@ -453,13 +455,17 @@ __global__ __launch_bounds__(TPB, DP <= 64 ? 2 : 1) void dkv_kernel(Args a, cons
   }
   if (j >= a.K) return;
   const int64_t row = (b * a.K + j) * a.Hk + kh, part = (int64_t)split * 2 * a.B * a.K * a.Hk;
-  if (a.splits > 1) {
-    store_row<DP>(a.part + (part + row) * D, dk, pow2i(-FK) * a.scale, D, half, a.vec);
-    store_row<DP>(a.part + (part + a.B * a.K * a.Hk + row) * D, dv, pow2i(-FV), D, half, a.vec);
-    return;
-  }
-  if (a.dk) store_row<DP>(a.dk + row * D, dk, pow2i(-FK) * a.scale, D, half, a.vec);
-  if (a.dv) store_row<DP>(a.dv + row * D, dv, pow2i(-FV), D, half, a.vec);
+  float* dk_out = a.splits > 1 ? a.part + (part + row) * D : a.dk ? a.dk + row * D : nullptr;
+  float* dv_out = a.splits > 1 ? a.part + (part + a.B * a.K * a.Hk + row) * D : a.dv ? a.dv + row * D : nullptr;
+  if (dk_out) store_row<DP>(dk_out, dk, pow2i(-FK) * a.scale, D, half, a.vec);
+  if (!dv_out) return;
+  store_row<DP>(dv_out, dv, pow2i(-FV), D, half, a.vec);
+  if (bad && in)
+    for (int u = u0; u < u1; ++u)
+      for (unsigned left = g_info[tile_of(u)].bad; left; left &= left - 1) {
+        const int64_t i = (int64_t)(qt0 + u % each) * kTile + __builtin_ctz(left);
+        if (!a.causal || j <= i + a.off) put_bad(a.go + ((b * a.Q + i) * a.H + kh * a.G + u / each) * D, D, half, dv_out);
+      }
 }
 
 // out[i] = sum over the parts of part[s][i], in order
@@ -549,7 +555,7 @@ int32_t dq_launch(Args a, hipStream_t s) {
   int32_t rc = allow_lds(dq_kernel<DP, BIAS>, lds);
   if (rc) return rc;
   const int64_t groups = ceil_div64(a.Q, 128) * a.H * a.B * a.splits;
-  hipLaunchKernelGGL((dq_kernel<DP, BIAS>), dim3((unsigned)groups), dim3(TPB), lds, s, a, a.k_shift, a.v_shift, a.meta);
+  hipLaunchKernelGGL((dq_kernel<DP, BIAS>), dim3((unsigned)groups), dim3(TPB), lds, s, a, a.k_info, a.v_info, a.meta);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }
@@ -560,7 +566,7 @@ int32_t dkv_launch(const Args& a, hipStream_t s) {
   int32_t rc = allow_lds(dkv_kernel<DP, BIAS>, lds);
   if (rc) return rc;
   const int64_t groups = ceil_div64(a.K, 128) * a.Hk * a.B * a.splits;
-  hipLaunchKernelGGL((dkv_kernel<DP, BIAS>), dim3((unsigned)groups), dim3(TPB), lds, s, a, a.q_shift, a.g_shift, a.meta);
+  hipLaunchKernelGGL((dkv_kernel<DP, BIAS>), dim3((unsigned)groups), dim3(TPB), lds, s, a, a.q_info, a.g_info, a.meta);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }

@@ -22,7 +22,7 @@ constexpr float kSlack = 4.f;  // p <= 2^kSlack
 constexpr int kPTop = 11;      // probabilities are scaled by up to 2^kPTop: 2^(kPTop + kSlack) fits fp16
 
 template <int DP, bool BIAS>
-__global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __restrict__ k_shift, const int* __restrict__ v_shift) {
+__global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const TileInfo* __restrict__ k_info, const TileInfo* __restrict__ v_info) {
   constexpr int STAGE = DP * 256;  // row image of k, column image of v
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* bias_lds = reinterpret_cast<float*>(smem + 2 * STAGE);
@@ -78,6 +78,7 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __re
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) o[d] = floatx16{};
   float m = -INFINITY, l = 0.f;
+  unsigned bad = 0;
   int F = 2 * kMaxShift;  // the output accumulator holds 2^F times the sums of p v
   if (t0 < t1) request(t0, 0);
   wait_loads();
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __re
           read_line(kimg + kb * 4096, col, st, half, kh8, kl8);
           s = mfma_pairs(kh8, kl8, qh[2 * kb + st], ql[2 * kb + st], s);
         }
-      const float c = cq * pow2i(-k_shift[tile_at + t]);
+      const float c = cq * pow2i(-k_info[tile_at + t].shift);
       const int key0 = t * kTile + 4 * half;
       float x[16];
 #pragma unroll
@@ -132,7 +133,8 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __re
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[d][v] *= keep;
       }
-      const int vs = v_shift[tile_at + t];
+      const int vs = v_info[tile_at + t].shift;
+      bad |= v_info[tile_at + t].bad;
       if (kPTop + vs < F) {
         if (F < 2 * kMaxShift) {
           const float down = pow2i(kPTop + vs - F);
@@ -180,9 +182,10 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __re
   if (!in) return;
   l += __shfl_xor(l, 32, 64);
   const float down = pow2i(-F);
+  const int64_t part = ((b * a.H + h) * a.Q + i) * a.splits + split;
+  float* out = a.splits == 1 ? a.o + ((b * a.Q + i) * a.H + h) * D : a.part + part * D;
   if (a.splits == 1) {
     const float inv = l != 0.f ? down / l : 0.f;
-    float* out = a.o + ((b * a.Q + i) * a.H + h) * D;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -199,19 +202,24 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const int* __re
       }
     if (half == 0 && a.lse) a.lse[(b * a.H + h) * a.Q + i] = l != 0.f ? (m + log2_fast(l)) * kLn2 : -INFINITY;
   } else {
-    const int64_t part = ((b * a.H + h) * a.Q + i) * a.splits + split;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const int at = d * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-        if (at < D) a.part[part * D + at] = o[d][v] * down;
+        if (at < D) out[at] = o[d][v] * down;
       }
     if (half == 0) {
       a.part_ml[2 * part] = m;
       a.part_ml[2 * part + 1] = l;
     }
   }
+  if (bad)
+    for (int t = t0; t < t1; ++t)
+      for (unsigned left = v_info[tile_at + t].bad; left; left &= left - 1) {
+        const int j = t * kTile + __builtin_ctz(left);
+        if (j < limit) put_bad(a.v + b * a.vs[0] + j * a.vs[1] + kh * a.vs[2], D, half, out);
+      }
 }
 
 template <int DP, bool BIAS>
@@ -220,7 +228,7 @@ int32_t launch(const Args& a, hipStream_t s) {
   const size_t lds = 2 * DP * 256 + (BIAS ? (2 * a.bk.near + 1) * 4 : 0);
   if (lds > 65536)
     ENDIA_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(forward_kernel<DP, BIAS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  hipLaunchKernelGGL((forward_kernel<DP, BIAS>), dim3((unsigned)groups), dim3(TPB), lds, s, a, a.k_shift, a.v_shift);
+  hipLaunchKernelGGL((forward_kernel<DP, BIAS>), dim3((unsigned)groups), dim3(TPB), lds, s, a, a.k_info, a.v_info);
   ENDIA_LAUNCH_CHECK();
   return ENDIA_HIP_OK;
 }

@@ -1430,8 +1430,9 @@ def attention(q, k, v, key_lengths=None, causal=False, scale=None, query_offset=
 
     heads is a multiple of key_heads, each of which serves that many query heads in a row. key_lengths: one whole number
     per batch entry, held as floats on the device; keys behind it are never read into a result, whatever they hold.
-    causal: query i sees the keys up to i + query_offset, so one new token over a cache of n tokens is query_offset = n.
-    scale defaults to dim ** -0.5. A query without any key left gives zeros, and zero gradients. dim is at most 128.
+    causal: query i sees the keys up to i + query_offset, so one new token over a cache of n tokens is query_offset = n; what the
+    keys behind hold does not reach it. scale defaults to dim ** -0.5. A query without any key left gives zeros, and zero
+    gradients. dim is at most 128.
     Views whose last axis is contiguous (slices of a fused projection) are read in place. First order only."""
     return _attention("attention", q, k, v, None, key_lengths, causal, scale, query_offset, 0)
 

@@ -431,8 +431,11 @@ ENDIA_API int32_t endia_hip_linear_cross_entropy_bwd(int64_t N, int64_t D, int64
  *      q [B, Q, H, D], k and v [B, K, Hk, D]: strides in elements for the batch, position and head axes, the last axis
  *      contiguous; H is a multiple of Hk, query head h reads key head h / (H / Hk). D <= ENDIA_ATTENTION_MAX_DIM.
  *      key_lengths: B whole numbers held as floats, or null: keys at and behind key_lengths[b] (clamped to 0 .. K) are
- *      left out and never take part, whatever they hold. causal: key j is left out of query i when j > i + query_offset.
- *      A query with no key left gets o = 0, lse = -inf and no gradient.
+ *      left out and never take part, whatever they hold. causal: key j is left out of query i when j > i + query_offset; what it
+ *      holds then reaches neither o nor a gradient through i (an infinity or NaN included). A query with no key left gets o = 0,
+ *      lse = -inf and no gradient, and gives none, whatever it and its cotangent hold. Infinities and NaN that take part give
+ *      infinities or NaN. Beyond 16 query rows per key head, and in every gradient, numbers are held to 2^-22 of their own size or
+ *      2^-38 of the largest in their 32 positions of one head, whichever is more.
  *      table [buckets, H] or null. A difference of n steps has bucket n for n < e (e = half the side's buckets), then
  *      e + floor(log(n/e) / log(max_distance/e) * (side - e)), at most side - 1. both_sides = 0: side = buckets, n counts
  *      back from the query, later keys have n = 0. both_sides = 1: side = buckets / 2, later keys use the second half.

@@ -115,6 +115,49 @@ def test_attention_queries_without_a_key_pass_nothing_on(Q, K):
             assert not got["dq"][:, :none].any()
 
 
+# ---- attention: a value that some queries of a tile see and others do not ------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("buckets", [None, 16])
+@pytest.mark.parametrize("T", [12, 40, 300])
+def test_attention_causal_nan_stays_behind_its_place(T, buckets):
+    """A NaN at place j reaches the queries from j on and the gradients of what they see; the queries before keep their values."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    for j in {0, 5, T // 2, T - 1}:
+        q, k, v, go = (rng.standard_normal((1, T, 2, 64)).astype(np.float32) for _ in range(4))
+        table = rng.standard_normal((buckets, 2)).astype(np.float32) if buckets else None
+        kw = dict(table=table, causal=True, max_distance=32)
+        want = attention_reference(q, k, v, go, **kw)
+
+        def check(got, name, nan, rest):
+            assert np.isnan(got[nan]).all(), (name, j)
+            within(got[rest], [a[rest] for a in want[name]], "%s, NaN at %d" % (name, j))
+
+        late, early, head1 = np.s_[:, j:, 0], np.s_[:, :j, 0], np.s_[:, :, 1]
+        bad = v.copy()
+        bad[0, j, 0, 5] = np.nan
+        o = attend(nd, q, k, bad, **kw)["o"]
+        check(o, "o", np.s_[:, j:, 0, 5], early)
+        within(np.delete(o, 5, 3), [np.delete(a, 5, 3) for a in want["o"]], "the other elements")
+        bad = k.copy()
+        bad[0, j, 0, 5] = np.nan
+        got = attend(nd, q, bad, v, go, **kw)
+        for n in ("o", "dq"):
+            check(got[n], n, late, early)
+            within(got[n][head1], [a[head1] for a in want[n]], n)
+        bad = q.copy()
+        bad[0, j, 0, 5] = np.nan
+        got = attend(nd, bad, k, v, go, **kw)
+        for n in ("dk", "dv"):
+            check(got[n], n, np.s_[:, :j + 1, 0], np.s_[:, j + 1:, 0])
+        bad = go.copy()
+        bad[0, j, 0, 5] = np.nan
+        got = attend(nd, q, k, v, bad, **kw)
+        check(got["dk"], "dk", np.s_[:, :j + 1, 0], np.s_[:, j + 1:, 0])
+        check(got["dv"], "dv", np.s_[:, :j + 1, 0, 5], np.s_[:, j + 1:, 0])
+        within(np.delete(got["dv"], 5, 3), [np.delete(a, 5, 3) for a in want["dv"]], "the other elements")
+
+
 # ---- attention: memory ----------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_attention_holds_the_cotangent_through_the_call(monkeypatch):
