@@ -215,11 +215,12 @@ struct Down {
 __device__ __forceinline__ void dx_block(const Direct& p, const floatx16& acc, int64_t r0, int left, int n, int half, int part) {
   if (n >= p.N) return;
   const Down down(mean_of(p.g, p.count));
+  const bool skip = p.target[n] < 0.f;  // (its cotangents are 0, but 0 times what the weight holds need not be)
   float* out = p.out + ((int64_t)part * p.N + n) * p.rows + r0;
 #pragma unroll
   for (int v = 0; v < 16; ++v) {
     const int i = k_of(half, v & 7) + 16 * (v >> 3);
-    const float y = down(acc[v]);
+    const float y = skip ? 0.f : down(acc[v]);
     if (i < left) out[i] = p.accumulate ? out[i] + y : y;
   }
 }

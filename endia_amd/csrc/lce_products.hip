@@ -397,6 +397,7 @@ __global__ __launch_bounds__(Tile<T>::TPB, 2) void gradient_kernel(Gradient p) {
   for (int j = 0; j < FB; ++j) {
     const int64_t bi = b0 + t.b_of(j);
     if (bi >= p.rows_b) continue;
+    const bool skip = p.left_out && p.left_out[bi] < 0.f;
 #pragma unroll
     for (int i = 0; i < FA; ++i)
 #pragma unroll
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(Tile<T>::TPB, 2) void gradient_kernel(Gradient p) {
         const int64_t ai = a0 + t.a_of(i, 4 * q);
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(acc[i][j][4 * q + e] * c.m, c.e - shift[j] - shift_of(p.a_amax[min(ai + e, p.rows_a - 1)]));
+        for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf((skip ? 0.f : acc[i][j][4 * q + e]) * c.m, c.e - shift[j] - shift_of(p.a_amax[min(ai + e, p.rows_a - 1)]));
         if (vec) {
           if (ai < p.rows_a) {
             float4* to = reinterpret_cast<float4*>(out + bi * p.ld + ai);

@@ -64,6 +64,7 @@ struct Gradient {
   int by_a, accumulate, parts, vec;  // (vec: set by gradient())
   int64_t part_stride;
   const float *g, *count;
+  const float* left_out;  // null, or per row of b a target: where it is negative the result is 0, whatever a holds
 };
 int32_t gradient(const Gradient& a, hipStream_t s);
 int product_tile(int64_t a, int64_t b);  // edge of the tiles that a product of a x b rows is cut into: 256 or 128

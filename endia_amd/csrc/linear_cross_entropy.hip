@@ -279,7 +279,9 @@ int32_t many_rows_bwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t l
       q.rows_a = D; q.rows_b = N; q.k = cols;
       q.out = parts > 1 ? w.at<float>(dxp) : dx;
       q.ld = D; q.by_a = 0; q.accumulate = v0 ? 1 : 0; q.parts = parts; q.part_stride = N * D;
+      q.left_out = target;
       if ((rc = lce::gradient(q, s))) return rc;
+      q.left_out = nullptr;
     }
     if (dW) {
       q.a = w.at<char>(xt); q.b = a.pt; q.a_amax = w.at<float>(xta); q.b_shift = a.pt_shift; q.b_shift_ld = ceil_div64(cols, lce::kPanel) * lce::kPanel;

@@ -226,3 +226,22 @@ def test_linear_cross_entropy_of_a_tiny_cotangent(N, tied):
         want, got = loss_reference(x, w, t, g), loss_of(nd, x, w, t, tied, g=g)
         for n in got:
             within(got[n], want[n], "%s with a cotangent of %g" % (n, g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("N", [9, 90, 600])
+def test_linear_cross_entropy_left_out_rows_get_no_gradient_from_a_broken_weight(N, tied):
+    """An infinity or NaN in the weight: the rows that count become NaN, those that are left out keep their zeros."""
+    import endia_amd as nd
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal((N, 40)).astype(np.float32), rng.standard_normal((40, 333)).astype(np.float32)
+    for value in (np.nan, np.inf):
+        bad = w.copy()
+        bad[3, 7] = value
+        for left in (np.arange(N) % 3 == 1, np.ones(N, bool)):
+            t = np.where(left, -1, 5).astype(np.float32)
+            got = loss_of(nd, x, bad, t, tied)
+            assert not got["dx"][left].any() and np.isnan(got["dx"][~left]).any(axis=1).all(), value
+            assert got["loss"][0] == 0 if left.all() else np.isnan(got["loss"][0])
+            assert np.isnan(got["dw"]).any() != left.all()
