@@ -9,8 +9,8 @@
 // p and ds are scaled per key (or query) by a running power of two, lowered with the accumulator when a block exceeds it.
 // Bound: the matrix pipe at DP = 128, the vector ALU at DP = 64 and below; with a table the 16 LDS additions of a tile near the
 // diagonal (half of dq's time at 512 keys). Measured, as fp32 products: 4096 queries x 16384 keys, 16 heads of 128: dq 2.62 ms = 315
-// TFLOP/s, dkv 3.76 ms = 293; 8 x 448 x 1500, 16 heads of 64: dq 122 us = 212, dkv 182 us = 189; 5001 causal with buckets: dq 813 us =
-// 189, dkv 1.07 ms = 192.
+// TFLOP/s, dkv 3.76 ms = 293; 8 x 448 x 1500, 16 heads of 64: dq 122 us = 212, dkv 182 us = 189; 5001 causal with buckets: dq 813 to
+// 822 us = 187 to 189, dkv 1.02 ms = 201.
 #include "attention.h"
 
 namespace attention {

@@ -9,7 +9,7 @@
 // straight into the other half of the LDS meanwhile.
 // Bound: the matrix pipe and the vector ALU about evenly (per 32 x 32 block 6 DP / 16 matrix instructions of 32 cycles and about
 // 20 vector instructions for each of 16 scores a lane). Measured, as fp32 products: 4096 queries x 16384 keys, 16 heads of 128: 1.46 ms =
-// 376 TFLOP/s; 8 x 448 x 1500, 16 heads of 64: 93 us = 185; 5001 causal, 16 heads of 128, with buckets: 394 us = 260.
+// 376 TFLOP/s; 8 x 448 x 1500, 16 heads of 64: 93 us = 185; 5001 causal, 16 heads of 128, with buckets: 394 to 404 us = 253 to 260.
 #include "attention.h"
 
 namespace attention {
@@ -145,8 +145,8 @@ __global__ __launch_bounds__(TPB, 2) void forward_kernel(Args a, const TileInfo*
         }
         F = kPTop + vs;
       }
-      // A tile whose v is 2^70 below the largest so far would leave no bits of p: below 2^-60 it is added as if it were larger,
-      // which is still nothing beside what is there.
+      // A tile whose v is 2^70 below the largest so far would leave no bits of p: below 2^-60 it is added as if it were larger. (What is
+      // below 2^-36 of the largest v so far is lost beside it: nothing to the rows that attend to that one too.)
       const int up = max(F - vs, -60);
       const float base = m == -INFINITY ? -INFINITY : m - (float)up;  // -inf: no key yet, exp2(-inf - -inf) is caught below
       float sum = 0.f;

@@ -7,9 +7,9 @@
 // instructions of 32 cycles against 48 LDS reads of 16 bytes a lane. The accumulator holds one b (a row of x, or a class) per lane
 // and four consecutive a per register quad, so that what is needed per row of x (maximum, sum, cotangent) stays within a lane but
 // for one exchange.
-// Bound: the matrix pipe. Measured at 8192 rows, width 4096, as fp32 products: statistics of 16384 classes 2.53 ms = 434 TFLOP/s (1.3
-// PFLOP/s of fp16 ones; a large library product reaches 1.17 on this card), cotangents of 4096 classes 722 us = 381, a gradient of them
-// 677 us = 406. Tiles of 128 x 128 reach about three quarters of that rate, two to a CU.
+// Bound: the matrix pipe. Measured at 8192 rows, width 4096, as fp32 products: statistics of 16384 classes 2.53 to 2.58 ms = 426 to 434
+// TFLOP/s (1.28 to 1.3 PFLOP/s of fp16 ones; a large library product reaches 1.17 on this card), cotangents of 4096 classes 722 to 732 us =
+// 376 to 381, a gradient of them 677 to 688 us = 400 to 406. Tiles of 128 x 128 reach about three quarters of that rate, two to a CU.
 #include "linear_cross_entropy.h"
 #include "mfma_tile.h"
 

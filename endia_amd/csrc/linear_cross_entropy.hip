@@ -128,8 +128,9 @@ int cut(int64_t tiles, int64_t want, int64_t steps, int64_t most) {
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------
-// From here on the weight is brought into panels. Both sides: 417 rows, 79335 classes x 1668 2.8 to 2.9 ms streamed, 3.1 to 3.8 in panels;
-// 512 rows, 65536 x 2048 2.8 to 2.9 and 2.7 to 2.9; 1000 rows, 30000 x 4096 4.9 to 5.0 and 3.8 to 4.0.
+// From here on the weight is brought into panels. Both sides, a step with the weight by class and by width: 417 rows, 79335 classes x
+// 1668 2.66 and 2.85 ms streamed, 3.22 and 3.61 in panels; 512 rows, 65536 x 2048 2.49 and 2.67, 2.68 and 2.93; 1000 rows, 30000 x 4096 4.33
+// and 4.65, 3.81 and 4.05.
 constexpr int64_t kManyRows = 512;
 
 int32_t few_rows_fwd(int64_t N, int64_t D, int64_t V, const float* x, int64_t ldx, int32_t transW, const float* W, int64_t ldw, const float* target,

@@ -435,7 +435,7 @@ ENDIA_API int32_t endia_hip_linear_cross_entropy_bwd(int64_t N, int64_t D, int64
  *      holds then reaches neither o nor a gradient through i (an infinity or NaN included). A query with no key left gets o = 0,
  *      lse = -inf and no gradient, and gives none, whatever it and its cotangent hold. Infinities and NaN that take part give
  *      infinities or NaN. Beyond 16 query rows per key head, and in every gradient, numbers are held to 2^-22 of their own size or
- *      2^-38 of the largest in their 32 positions of one head, whichever is more.
+ *      2^-38 of the largest in their 32 positions of one head, whichever is more, and o to 2^-36 of the head's largest value.
  *      table [buckets, H] or null. A difference of n steps has bucket n for n < e (e = half the side's buckets), then
  *      e + floor(log(n/e) / log(max_distance/e) * (side - e)), at most side - 1. both_sides = 0: side = buckets, n counts
  *      back from the query, later keys have n = 0. both_sides = 1: side = buckets / 2, later keys use the second half.
